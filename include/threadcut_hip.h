@@ -371,6 +371,26 @@ int tc_paged_append_rows(const void* const* k_rows_host, const int64_t k_strides
                          const int64_t* slots_dev, int num_layers, int batch, int heads, int64_t rows,
                          int head_dim, int dtype, void* stream);
 
+/* The same with the position rotation on the way: the keys arrive as their
+ * projection left them and are rotated to their positions (the rotation of
+ * threadcut/kv.py:20-25 by position * inv_freq, the angle reduced in 64 bits),
+ * the values are copied. Token r of batch row b goes to slots_dev[b][r] =
+ * {page, slot, position, 0} (int32 [batch, rows, 4] on the device, 16-byte
+ * aligned); a slot outside the pool is skipped. q_heads > 0: the queries of the
+ * same tokens ([batch, q_heads, rows, head_dim] per layer) are rotated into
+ * q_out_host's buffers, whatever their slots (0: the four q arguments are not
+ * read). inv_freq: head_dim / 2 floats, on the host (taken by value) or on the
+ * device; exactly one of the two pointers is set. */
+int tc_paged_append_rope(const void* const* k_rows_host, const int64_t k_strides[3],
+                         const void* const* v_rows_host, const int64_t v_strides[3],
+                         void* const* k_pools_host, void* const* v_pools_host,
+                         const int64_t pool_strides[3], int num_pages, int page_tokens,
+                         const int32_t* slots_dev, const void* const* q_rows_host,
+                         const int64_t q_strides[3], void* const* q_out_host,
+                         const int64_t q_out_strides[3], int q_heads, const float* inv_freq_host,
+                         const float* inv_freq_dev, int num_layers, int batch, int kv_heads,
+                         int64_t rows, int head_dim, int dtype, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Prefill attention                                                         */
 /* ------------------------------------------------------------------------ */

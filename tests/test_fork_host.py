@@ -1,0 +1,118 @@
+"""Pages shared by several sequences (PageTable.fork) against a brute-force model, and the argument checks of rotated
+appends, on the CPU."""
+import ctypes
+import random
+
+import pytest
+
+from threadcut_amd import _lib
+from threadcut_amd.paged import PageTable, _placed
+
+
+def check(t, model):
+    """Every sequence reads its own tokens, whatever the others wrote since: model[b] is its list of token names, and
+    `written` what each slot holds."""
+    for b, tokens in enumerate(model["tokens"]):
+        got = [model["written"][tuple(x)] for x in t.token_slots(b).tolist()]
+        assert got == tokens
+    users = {}
+    for b in range(t.batch):
+        for p in set(t.frags[b][:, 0].tolist()):
+            users[p] = users.get(p, 0) + 1
+    assert sorted(t.free) == sorted(set(range(t.num_pages)) - set(users))
+    assert len(set(t.free)) == len(t.free)
+    assert t.users == {p: n for p, n in users.items() if n > 1}
+
+
+@pytest.mark.parametrize("page_tokens", [16, 40, 64])
+@pytest.mark.parametrize("seed", range(8))
+def test_forks_match_brute_force(seed, page_tokens):
+    rnd = random.Random(seed)
+    t = PageTable(300, page_tokens, batch=5)
+    model = {"tokens": [[] for _ in range(5)], "written": {}}
+    name = 0
+    for _ in range(150):
+        b = rnd.randrange(5)
+        tokens = model["tokens"][b]
+        what = rnd.random()
+        if what < 0.45:
+            n = rnd.choice([1, 1, 5, 16, 30, rnd.randint(1, 150)])
+            if t.pages_needed(b, n) > len(t.free):
+                with pytest.raises(RuntimeError, match="pages needed"):
+                    t.reserve(b, n)
+                continue
+            free = len(t.free)
+            need = t.pages_needed(b, n)
+            for slot in t.reserve(b, n).tolist():
+                model["written"][tuple(slot)] = name  # a slot that another sequence reads would change its token
+                tokens.append(name)
+                name += 1
+            assert free - len(t.free) == need
+        elif what < 0.7:
+            src = rnd.randrange(5)
+            n = rnd.randint(0, len(model["tokens"][src]))
+            if src == b or tokens:
+                with pytest.raises(ValueError, match="empty"):
+                    t.fork(src, b, n)
+                continue
+            t.fork(src, b, n)
+            model["tokens"][b] = model["tokens"][src][:n]
+        elif what < 0.88:
+            a = rnd.randint(0, len(tokens))
+            c0 = rnd.randint(a, len(tokens))
+            c = rnd.randint(0, len(tokens) - c0)
+            t.prune(b, a, c0, c)
+            model["tokens"][b] = tokens[:a] + tokens[c0:c0 + c]
+        else:
+            t.release(b)
+            model["tokens"][b] = []
+        check(t, model)
+    for b in range(5):
+        t.release(b)
+    assert len(t.free) == 300 and not t.users
+
+
+def test_fork_refusals():
+    t = PageTable(8, 16, batch=3)
+    t.reserve(0, 20)
+    for src, dst, n, match in ((0, 0, 5, "empty"), (0, 1, 21, "21 tokens"), (0, 1, -1, "tokens")):
+        with pytest.raises(ValueError, match=match):
+            t.fork(src, dst, n)
+    t.fork(0, 1, 0)  # nothing shared
+    assert t.length(1) == 0 and not t.users
+    t.fork(0, 1, 20)
+    with pytest.raises(ValueError, match="empty"):
+        t.fork(0, 1, 20)
+    assert t.reserve(0, 1).tolist() == [[2, 0]]  # neither writes behind the other's last token
+    assert t.reserve(1, 1).tolist() == [[3, 0]]
+
+
+def test_rotated_append_validation():
+    lib = _lib.load()
+    st = _lib.i64x3(0, 1 << 20, 128)
+    p, f = _lib.ptr_array([4096]), (ctypes.c_float * 64)()
+    pool = _lib.i64x3(8 * 16 * 128, 16 * 128, 128)
+
+    def rope(k=p, ks=st, slots=4096, pages=4, P=16, q=None, qs=None, qo=None, hq=0, host=f, dev=None, layers=1, b=1, h=8,
+             rows=3, d=128, dt=0, ps=pool):
+        return lib.tc_paged_append_rope(k, ks, p, st, p, p, ps, pages, P, slots, q, qs, qo, qs, hq, host, dev, layers,
+                                        b, h, rows, d, dt, None)
+
+    assert rope(slots=None) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(slots=4104) == _lib.TC_ERR_ALIGNMENT
+    assert rope(pages=0) == rope(P=0) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(host=None) == _lib.TC_ERR_INVALID_ARGUMENT and b"frequencies" in lib.tc_last_error()
+    assert rope(dev=4096) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(host=None, dev=4098) == _lib.TC_ERR_ALIGNMENT
+    assert rope(k=_lib.ptr_array([0])) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(k=_lib.ptr_array([4100])) == _lib.TC_ERR_ALIGNMENT
+    assert rope(ks=_lib.i64x3(0, 1 << 20, 130)) == _lib.TC_ERR_ALIGNMENT
+    assert rope(ps=_lib.i64x3(0, 0, 64)) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(hq=8) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(hq=8, q=p, qs=st, qo=_lib.ptr_array([0])) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(d=64) == rope(dt=5) == _lib.TC_ERR_UNSUPPORTED
+    assert rope(b=0) == rope(layers=-1) == rope(rows=-1) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert rope(rows=1 << 30, b=4) == _lib.TC_ERR_UNSUPPORTED
+    assert rope(h=40000) == _lib.TC_ERR_UNSUPPORTED
+    assert rope(rows=0, slots=None, host=None) == rope(layers=0, slots=None) == _lib.TC_OK
+    assert _placed([[4, 1], [5, 0]], 7).tolist() == [[4, 1, 7, 0], [5, 0, 8, 0]]

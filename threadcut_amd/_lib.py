@@ -76,6 +76,8 @@ SIGNATURES = {
     "tc_append_rows": (_I, [_P, _I64P, _P, _I64P, _P, _P, _I64P, _I64, _I64, _I, _I, _I64, _I, _I, _P]),
     "tc_paged_append_rows": (_I, [_PP, _I64P, _PP, _I64P, _PP, _PP, _I64P, _I, _I, _P, _I, _I, _I, _I64, _I, _I,
                                   _P]),
+    "tc_paged_append_rope": (_I, [_PP, _I64P, _PP, _I64P, _PP, _PP, _I64P, _I, _I, _P, _PP, _I64P, _PP, _I64P, _I, _FP,
+                                  _P, _I, _I, _I, _I64, _I, _I, _P]),
     "tc_prefill_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _P, _S, _I, _I64, _I64, _I, _I,
                                   _I, _I, _I, _F, _I, _P, _S, _P, _I64P, _P]),
     "tc_prefill_paged_attention": (_I, [_P, _I64P, _P, _P, _I64P, _I, _P, _I64, _P, _I64P, _P, _S, _I, _I64, _I64,

@@ -93,4 +93,29 @@ __device__ __forceinline__ float row_bcast(float x) {
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
+// out = fp(fl(x*cos) + fl(rotate_half(x)*sin)) per element, no contraction:
+// lower half  y = x_lo*cos - x_hi*sin,  upper half y = x_hi*cos + x_lo*sin.
+template <int DT>
+__device__ __forceinline__ void rotate_pair(uint4& lo, uint4& hi, const float (&cv)[8], const float (&sv)[8]) {
+#pragma clang fp contract(off)
+  using E = Elem<DT>;
+  uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w};
+  uint32_t wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float c0 = cv[2 * w], c1 = cv[2 * w + 1];
+    const float s0 = sv[2 * w], s1 = sv[2 * w + 1];
+    const float xl0 = E::lo(wl[w]), xl1 = E::hi(wl[w]);
+    const float xh0 = E::lo(wh[w]), xh1 = E::hi(wh[w]);
+    const float yl0 = xl0 * c0 - xh0 * s0;
+    const float yl1 = xl1 * c1 - xh1 * s1;
+    const float yh0 = xh0 * c0 + xl0 * s0;
+    const float yh1 = xh1 * c1 + xl1 * s1;
+    wl[w] = E::bits(yl0) | (E::bits(yl1) << 16);
+    wh[w] = E::bits(yh0) | (E::bits(yh1) << 16);
+  }
+  lo = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+  hi = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+}
+
 }  // namespace tc

@@ -38,7 +38,7 @@ from transformers.cache_utils import DynamicLayer
 
 from . import _lib
 from .flash_decode import HEAD_DIM, _on_device, _plan
-from .kv import rope_table, rows_ok, watched
+from .kv import _plain, rope_table, rotate_half, rows_ok, watched
 from .prefill import GROUPS
 
 TILE = 16  # rows per tile-table entry (the decode kernel's tile)
@@ -84,6 +84,20 @@ def _addr(a):
     return a.__array_interface__["data"][0]
 
 
+def _rotated(x, positions, inv_freq):
+    """x [B, heads, n, 128] rotated to int positions [B, n] by torch operations: the angles in 64 bits, the rotation in
+    fp32, the result in x's type (what tc_paged_append_rope computes)."""
+    angle = positions[..., None].double() * inv_freq.to(x.device).float().double()
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+    f = x.float()
+    return (f * torch.cat((cos, cos), -1) + rotate_half(f) * torch.cat((sin, sin), -1)).to(x.dtype)
+
+
+def _rows_strides(t):
+    """(batch, head, token) strides of [B, heads, n, D] rows."""
+    return _lib.i64x3(*t.stride()[:3])
+
+
 def _frag_arg(frags):
     f = frags
     if not (isinstance(f, np.ndarray) and f.dtype == np.int64 and f.ndim == 2 and f.flags.c_contiguous):
@@ -114,6 +128,27 @@ def tiles_of(frags, page_tokens):
     return np.ascontiguousarray(_tiles(frags, page_tokens)[:, :3])
 
 
+def _placed(slots, start):
+    """int64 [n, 2] slots of consecutive tokens as int32 [n, 4] rows (page, slot, position, 0), the first at `start`."""
+    out = np.zeros((len(slots), 4), dtype=np.int32)
+    out[:, :2] = slots
+    out[:, 2] = np.arange(start, start + len(slots))
+    return out
+
+
+def _check_inv_freq(f, what):
+    if not isinstance(f, torch.Tensor) or f.shape != (HEAD_DIM // 2,) or not f.is_floating_point():
+        raise ValueError(f"PagedKV.{what}: inv_freq must be a float tensor of {HEAD_DIM // 2} inverse frequencies")
+
+
+def _query_ok(t, pool, rows):
+    """rows_ok for the query heads of new tokens (any number of heads)."""
+    sh, st = t.shape, t.stride()
+    return (t.is_cuda and len(sh) == 4 and sh[3] == HEAD_DIM and sh[2] == rows and t.dtype == pool.dtype
+            and t.get_device() == pool.get_device() and st[3] == 1 and not (st[0] | st[1] | st[2]) & 7
+            and not t.data_ptr() & 15 and _plain(t))
+
+
 class PageTable:
     """Pages of `page_tokens` slots shared by `batch` sequences (host bookkeeping).
 
@@ -127,6 +162,7 @@ class PageTable:
         self.page_tokens = int(page_tokens)
         self.free = list(range(self.num_pages - 1, -1, -1))  # pop() hands out the lowest id first
         self.frags = [_EMPTY.copy() for _ in range(batch)]
+        self.users = {}  # pages that more than one sequence uses (fork): how many do
         self.version = 0  # bumped on every change, so device copies know when to refresh
 
     @property
@@ -136,13 +172,49 @@ class PageTable:
     def length(self, b):
         return int(self.frags[b][:, 2].sum())
 
+    def _room(self, b):
+        """Slots that sequence b's next tokens find on its last page (none on a shared one: the others' tokens are,
+        or will be, behind its own)."""
+        fr = self.frags[b]
+        if len(fr) == 0 or int(fr[-1, 0]) in self.users:
+            return 0
+        return int(self.page_tokens - fr[-1, 1] - fr[-1, 2])
+
+    def _drop(self, pages):
+        """Takes one user from each of `pages`; returns those that nobody uses any more."""
+        freed = []
+        for p in pages:
+            n = self.users.pop(p, 1) - 1
+            if n > 1:
+                self.users[p] = n
+            elif n == 0:
+                freed.append(p)
+        return freed
+
+    def fork(self, src, dst, n):
+        """Sequence dst (empty) starts with the first n tokens of sequence src, in the same pages. They stay where
+        they are until the last of the sequences that use them lets them go."""
+        if src == dst or len(self.frags[dst]):
+            raise ValueError(f"fork: sequence {dst} is not an empty one beside sequence {src}")
+        if not 0 <= n <= self.length(src):
+            raise ValueError(f"fork: {n} tokens of a sequence of {self.length(src)}")
+        fr = _cut(self.frags[src], 0, n)
+        for p in set(fr[:, 0].tolist()):
+            self.users[p] = self.users.get(p, 1) + 1
+        self.frags[dst] = fr.copy()
+        self.version += 1
+
+    def pages_needed(self, b, n):
+        """Pages that the next n tokens of sequence b take from the free list."""
+        return -(-max(0, n - self._room(b)) // self.page_tokens)
+
     def reserve(self, b, n):
         """Slots of the next n tokens of sequence b, in order: int64 [n, 2] of (page, slot)."""
         if n < 0:
             raise ValueError("reserve: n must be >= 0")
         P = self.page_tokens
         fr = self.frags[b]
-        room = int(P - fr[-1, 1] - fr[-1, 2]) if len(fr) else 0
+        room = self._room(b)
         take = min(n, room)
         rest = n - take
         k = -(-rest // P)
@@ -182,14 +254,14 @@ class PageTable:
         _lib.check(rc, "tc_page_prune")
         nk, ns, nfr = (int(x) for x in buf[7 * nf + 3:])
         self.frags[b] = buf[:3 * nk].reshape(nk, 3).copy()
-        freed = buf[6 * nf + 3:6 * nf + 3 + nfr].tolist()
+        freed = self._drop(buf[6 * nf + 3:6 * nf + 3 + nfr].tolist())
         self.free += freed[::-1]
         self.version += 1
         return buf[3 * nf + 3:3 * nf + 3 + 3 * ns].reshape(ns, 3).copy(), freed
 
     def release(self, b):
-        """Drop sequence b entirely (its pages return to the free list)."""
-        self.free += sorted(set(self.frags[b][:, 0].tolist()), reverse=True)
+        """Drop sequence b entirely (the pages that no other sequence shares return to the free list)."""
+        self.free += sorted(self._drop(set(self.frags[b][:, 0].tolist())), reverse=True)
         self.frags[b] = _EMPTY.copy()
         self.version += 1
 
@@ -266,18 +338,29 @@ class PagedKV:
     def _strides(self):
         return _lib.i64x3(*self.k_pools[0].stride()[:3])
 
-    def append(self, b, ks, vs):
+    def append(self, b, ks, vs, inv_freq=None):
         """Append tokens to sequence b: ks/vs are per-layer [Hkv, n, D] (or
-        [1, Hkv, n, D]) tensors on the pools' device."""
+        [1, Hkv, n, D]) tensors on the pools' device. With ``inv_freq`` (float [D / 2])
+        the keys are not rotated yet: they are rotated to their positions, length(b)
+        onwards, on the way into their slots."""
         if len(ks) != self.layers or len(vs) != self.layers:
             raise ValueError(f"append: {self.layers} layers of K and V expected")
         n = ks[0].shape[-2]
         for t in list(ks) + list(vs):
             if t.shape[-2] != n or t.numel() != self.kv_heads * n * HEAD_DIM:
                 raise ValueError(f"append: every layer's K and V must be [{self.kv_heads}, {n}, {HEAD_DIM}]")
+        if inv_freq is not None:
+            _check_inv_freq(inv_freq, "append")
+        start = self.table.length(b)
         slots = self.table.reserve(b, n)
         if n == 0:
             return
+        if inv_freq is not None and self.layers:
+            ks, vs = [_as_batch(t) for t in ks], [_as_batch(t) for t in vs]
+            at = _to_device(_placed(slots, start)[None], self.device)
+            if self._write_rotated(range(self.layers), ks, vs, at, inv_freq):
+                return
+            ks = [_rotated(t.reshape(1, self.kv_heads, n, HEAD_DIM), at[..., 2], inv_freq) for t in ks]
         idx = _to_device(slots, self.device)
         if self.layers and self._write_rows(range(self.layers), [_as_batch(t) for t in ks], [_as_batch(t) for t in vs],
                                             idx):
@@ -314,6 +397,37 @@ class PagedKV:
         increment_version([pools[i] for i in layers for pools in (self.k_pools, self.v_pools)])
         return True
 
+    def _write_rotated(self, layers, ks, vs, slots, inv_freq, qs=(), q_outs=()):
+        """New tokens' rows, per layer [B, Hkv, n, D], into the pools' slots (int32 [B, n, 4] of (page, slot, position,
+        0) on the device), the keys rotated to their positions, and the queries qs of the same tokens, rotated, into
+        q_outs (per layer [B, Hq, n, D]), with one launch (tc_paged_append_rope). False if the kernel does not take the
+        tensors: nothing is written then."""
+        if watched():
+            return False
+        b, n = slots.shape[:2]
+        for group, pools, ok in ((ks, self.k_pools, rows_ok), (vs, self.v_pools, rows_ok), (qs, self.k_pools, _query_ok)):
+            for i, t in zip(layers, group):
+                if t.shape[0] != b or t.stride() != group[0].stride() or not ok(t, pools[i], n):
+                    return False
+        pool, dev = self.k_pools[0], inv_freq.is_cuda
+        f = inv_freq.to(self.device if dev else "cpu", torch.float32).contiguous()
+        heads = qs[0].shape[1] if len(qs) else 0
+        with _on_device(self.device):
+            rc = _lib.load().tc_paged_append_rope(
+                _lib.ptr_array([t.data_ptr() for t in ks]), _rows_strides(ks[0]),
+                _lib.ptr_array([t.data_ptr() for t in vs]), _rows_strides(vs[0]),
+                _lib.ptr_array([self.k_pools[i].data_ptr() for i in layers]),
+                _lib.ptr_array([self.v_pools[i].data_ptr() for i in layers]), self._strides(), pool.shape[0],
+                pool.shape[2], slots.data_ptr(),
+                _lib.ptr_array([t.data_ptr() for t in qs]) if heads else None, _rows_strides(qs[0]) if heads else None,
+                _lib.ptr_array([t.data_ptr() for t in q_outs]) if heads else None,
+                _rows_strides(q_outs[0]) if heads else None, heads, None if dev else _lib.float_array(f),
+                f.data_ptr() if dev else None, len(ks), b, self.kv_heads, n, HEAD_DIM, _lib.dtype_code(self.dtype),
+                _lib.stream_of(self.device))
+        _lib.check(rc, "tc_paged_append_rope")
+        increment_version([pools[i] for i in layers for pools in (self.k_pools, self.v_pools)])
+        return True
+
     def gather(self, layer, b=0):
         """Sequence b's K and V of one layer in logical order, [Hkv, n, D] copies."""
         slots = self.table.token_slots(b)
@@ -324,6 +438,13 @@ class PagedKV:
         k = self.k_pools[layer][idx[:, 0], :, idx[:, 1]].transpose(0, 1).contiguous()
         v = self.v_pools[layer][idx[:, 0], :, idx[:, 1]].transpose(0, 1).contiguous()
         return k, v
+
+    def fork(self, src, dst, n=None):
+        """Sequence dst (empty) starts with the first n tokens (default: all) of sequence src, in the same
+        pages: nothing is copied, and decode() reads what all sequences share once for all of them. Both grow
+        on pages of their own. Shared tokens can be dropped by each sequence; prune() does not move them."""
+        self._refuse_during_step("fork")
+        self.table.fork(src, dst, self.table.length(src) if n is None else n)
 
     def device_table(self):
         """(tile table int32 [B, max_tiles, 4], tiles int32 [B], max_tiles) on the device."""
@@ -424,12 +545,12 @@ class PagedKV:
                                "every layer (or cancel_step()) first")
 
     def cancel_step(self):
-        """Drop the slots of an incomplete reserved step (each sequence's last token)."""
+        """Drop the slots of an incomplete reserved step (each sequence's last tokens)."""
         if not self._step_pending():
             return
         for b in range(self.table.batch):
             n = self.table.length(b)
-            self.table.prune(b, n - 1, n, 0)
+            self.table.prune(b, n - self._step[2], n, 0)
         self._step = None
 
     def decode(self, layer, q, scale, out=None, split=None):
@@ -467,31 +588,69 @@ class PagedKV:
             _lib.check(rc, "tc_decode_paged_attention")
         return out
 
-    def reserve_step(self):
-        """Reserve one slot per sequence for the next decode token (once per step,
-        before layer 0); every layer's `decode_append` of that step then writes
-        its new K/V row there."""
+    def reserve_step(self, n=1):
+        """Reserve the slots of the next n tokens of every sequence (once per step,
+        before layer 0); every layer's `decode_append` (one token) or `write_step` of that
+        step then writes its new K/V rows there. Without room for all of them nothing is
+        reserved."""
+        if n < 1:
+            raise ValueError(f"PagedKV.reserve_step: {n} tokens")
         self._refuse_during_step("reserve_step")
+        need = sum(self.table.pages_needed(b, n) for b in range(self.table.batch))
+        if need > len(self.table.free):
+            raise RuntimeError(f"PagedKV.reserve_step: {need} pages needed, {len(self.table.free)} free")
+        slots = []
         for b in range(self.table.batch):
-            self.table.reserve(b, 1)
-        self._step = (self.table.version, set(range(self.layers)))
+            start = self.table.length(b)
+            slots.append(_placed(self.table.reserve(b, n), start))
+        # (table version, layers not written yet, tokens, the slots and their copy for each stream)
+        self._step = (self.table.version, set(range(self.layers)), int(n), np.stack(slots), {})
 
-    def write_step(self, layer, k_new, v_new):
-        """The unfused order of a decode step: write one layer's new K/V rows ([B, Hkv, D] or
-        [B, Hkv, 1, D]) into the slots reserve_step() took, with two torch row copies. Once a
-        layer's row is written (here or by decode_append), decode() and prefill() of that layer
-        read the new token; prune() and the next reserve_step() wait for every layer."""
+    def write_step(self, layer, k_new, v_new, inv_freq=None, query=None):
+        """The unfused order of a step: write one layer's new K/V rows ([B, Hkv, n, D], or
+        [B, Hkv, D] of one token) into the slots reserve_step(n) took. Once a layer's rows
+        are written (here or by decode_append), decode() and prefill() of that layer read the
+        new tokens; prune() and the next reserve_step() wait for every layer.
+
+        With ``inv_freq`` (float [D / 2]) the keys are not rotated yet: they are rotated to
+        their positions on the way, and so are the tokens' queries, if given ([B, Hq, n, D];
+        returned as a new tensor of that shape)."""
         step = getattr(self, "_step", None)
         if step is None or step[0] != self.table.version or layer not in step[1]:
             raise RuntimeError(f"PagedKV.write_step: layer {layer} has no reserved slot in this step")
-        b = self.table.batch
-        kn = k_new.reshape(b, self.kv_heads, HEAD_DIM)
-        vn = v_new.reshape(b, self.kv_heads, HEAD_DIM)
-        for i in range(b):
-            page, slot = (int(x) for x in self.table.token_slots(i)[-1])
-            self.k_pools[layer][page, :, slot] = kn[i]
-            self.v_pools[layer][page, :, slot] = vn[i]
+        b, n = self.table.batch, step[2]
+        kn = k_new.reshape(b, self.kv_heads, n, HEAD_DIM)
+        vn = v_new.reshape(b, self.kv_heads, n, HEAD_DIM)
+        out = None
+        if inv_freq is not None:
+            _check_inv_freq(inv_freq, "write_step")
+        if query is not None:
+            if inv_freq is None:
+                raise ValueError("PagedKV.write_step: a query is rotated by inv_freq, which is missing")
+            if query.dim() != 4 or query.shape[0] != b or query.shape[2:] != (n, HEAD_DIM) or \
+                    query.dtype != self.dtype or query.device != self.device:
+                raise ValueError(f"PagedKV.write_step: query {tuple(query.shape)} {query.dtype} on {query.device}, "
+                                 f"expected [{b}, Hq, {n}, {HEAD_DIM}] {self.dtype} on {self.device}")
+        done = False
+        if inv_freq is not None:
+            if torch.cuda.is_current_stream_capturing():  # (a replay would write this step's slots again)
+                raise RuntimeError("PagedKV.write_step: rotated rows are not captured; decode_append_at is")
+            at = _lib.per_stream(step[4], self.device.index, lambda: _to_device(step[3], self.device))
+            if query is not None:
+                out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            done = self._write_rotated([layer], [kn], [vn], at, inv_freq, *(([query], [out]) if query is not None else ()))
+            if not done:
+                kn = _rotated(kn, at[..., 2], inv_freq)
+                out = _rotated(query, at[..., 2], inv_freq) if query is not None else None
+        if not done:
+            for i, slots in enumerate(step[3]):  # a run of slots of one page at a time
+                ends = np.flatnonzero(np.diff(slots[:, 0])) + 1
+                for lo, hi in zip([0, *ends.tolist()], [*ends.tolist(), n]):
+                    page, first = int(slots[lo, 0]), int(slots[lo, 1])
+                    self.k_pools[layer][page, :, first:first + hi - lo] = kn[i, :, lo:hi]
+                    self.v_pools[layer][page, :, first:first + hi - lo] = vn[i, :, lo:hi]
         step[1].discard(layer)
+        return out
 
     def decode_append(self, layer, q, k_new, v_new, scale, out=None, split=None):
         """One decode step of one layer with the append fused in: k_new/v_new
@@ -499,6 +658,8 @@ class PagedKV:
         attends every key of its sequence including the new one. Returns out
         [B, Hkv, G, D]."""
         step, fast = getattr(self, "_step", None), _lib.FAST
+        if step is not None and step[2] != 1 and step[0] == self.table.version:
+            raise RuntimeError(f"PagedKV.decode_append: the step has {step[2]} tokens a sequence (write_step takes them)")
         if (fast is not None and split is None and q.is_cuda and step is not None and step[0] == self.table.version
                 and layer in step[1]):
             # The whole call in native code; None for what it does not take (then as below).
@@ -585,8 +746,13 @@ class PagedKV:
         re-rotated in place by -(c0 - a) positions in every layer. Returns the
         freed page ids."""
         self._refuse_during_step("prune")
-        suffix, freed = self.table.prune(b, s.a, s.c0, s.c)
         gap = s.c0 - s.a
+        if gap and self.table.users:
+            kept = _cut(self.table.frags[b], s.c0, s.c0 + s.c)[:, 0].tolist()
+            if any(p in self.table.users for p in kept):
+                raise RuntimeError(f"PagedKV.prune: tokens [{s.c0}, {s.c0 + s.c}) of sequence {b} would move, and other "
+                                   "sequences share their pages")
+        suffix, freed = self.table.prune(b, s.a, s.c0, s.c)
         tiles = tiles_of(suffix, self.table.page_tokens)
         if gap and len(tiles):
             t = np.zeros((len(tiles), 4), dtype=np.int32)
