@@ -396,7 +396,7 @@ def _own(st):
                 q = cache.decode(i, q.reshape(b, hkv, -1, D), SCALE, window=window,
                                  sink_tokens=sinks).reshape(b, 1, -1, D)
             outs.append(q)
-    for i, n in enumerate(st["counts"]):  # the tokens are taken back (a rejected draft)
+    for i, n in reversed(list(enumerate(st["counts"]))):  # the tokens are taken back, the last page taken first
         cache.prune(i, Split(n, cache.length(i), 0), st["inv_freq"])
     return {"k": cache.k_pools, "v": cache.v_pools, "out": outs}
 
