@@ -147,6 +147,25 @@ int tc_decode_attention(const void* q_dev, const int64_t q_strides[3],
                         void* workspace_dev, size_t workspace_bytes,
                         void* out_dev, const int64_t out_strides[3], void* stream);
 
+/* tc_decode_attention with a sliding window: the query, at the last of its
+ * sequence's tokens, sees the last `window` of them (its own included) and the
+ * first sink_tokens; no others are read. window >= 1, sink_tokens >= 0. The
+ * split plan and the workspace are those of tc_decode_window_tokens tokens.
+ * No counterpart in the reference (its models attend the whole cache). */
+int tc_decode_window_attention(const void* q_dev, const int64_t q_strides[3],
+                               const void* k_dev, const int64_t k_strides[3],
+                               const void* v_dev, const int64_t v_strides[3],
+                               const int32_t* lens_dev, int64_t n_tokens,
+                               int64_t window, int64_t sink_tokens,
+                               int batch, int kv_heads, int group, int head_dim,
+                               int dtype, float scale, int split_tokens,
+                               void* workspace_dev, size_t workspace_bytes,
+                               void* out_dev, const int64_t out_strides[3], void* stream);
+
+/* Tokens that tc_decode_num_splits is asked about for a windowed call (the
+ * visible ones, the sinks in whole tiles of 16), or a negative TC_ERR_* code. */
+int64_t tc_decode_window_tokens(int64_t n_tokens, int64_t window, int64_t sink_tokens);
+
 /* Bytes of the static scratch array of tc_decode_attention_noalloc (per GPU). */
 #define TC_DECODE_SCRATCH_BYTES (8u << 20)
 
@@ -212,6 +231,22 @@ int tc_decode_append_attention_at(const void* q_dev, const int64_t q_strides[3],
                                   float scale, int split_tokens,
                                   void* workspace_dev, size_t workspace_bytes,
                                   void* out_dev, const int64_t out_strides[3], void* stream);
+
+/* The two calls before with a sliding window: the new token's query sees the
+ * last `window` tokens, the new one among them, and the first sink_tokens.
+ * pos_dev NULL: n_tokens counts the new token (tc_decode_append_attention);
+ * else n_tokens is the capacity (tc_decode_append_attention_at). Workspace as
+ * tc_decode_window_attention of n_tokens tokens with one length. */
+int tc_decode_append_window_attention(const void* q_dev, const int64_t q_strides[3],
+                                      void* k_cache_dev, const int64_t k_strides[3],
+                                      void* v_cache_dev, const int64_t v_strides[3],
+                                      const void* k_new_dev, const int64_t k_new_strides[2],
+                                      const void* v_new_dev, const int64_t v_new_strides[2],
+                                      const int32_t* pos_dev, int64_t n_tokens, int64_t window,
+                                      int64_t sink_tokens, int batch, int kv_heads, int group,
+                                      int head_dim, int dtype, float scale, int split_tokens,
+                                      void* workspace_dev, size_t workspace_bytes, void* out_dev,
+                                      const int64_t out_strides[3], void* stream);
 
 /* Decode over a paged cache. k_pool_dev / v_pool_dev are page pools
  * [num_pages, kv_heads, page_tokens, head_dim] with element strides
@@ -445,6 +480,35 @@ int tc_prefill_paged_attention(const void* q, const int64_t q_strides[3],
                                int head_dim, int dtype, float scale,
                                int num_splits, void* workspace, size_t workspace_bytes,
                                void* out, const int64_t out_strides[3], void* stream);
+
+/* tc_prefill_attention with causal = 1 and a sliding window: the query at
+ * position p (the queries are the last of the n_tokens) sees keys j <= p with
+ * j > p - window or j < sink_tokens. Tiles that no row sees are not read.
+ * window >= 1, sink_tokens >= 0. num_splits as tc_prefill_window_num_splits
+ * returns it (0: the same), workspace as tc_prefill_workspace_bytes. */
+int tc_prefill_window_attention(const void* q_dev, const int64_t q_strides[3],
+                                const void* k_dev, const int64_t k_strides[3],
+                                const void* v_dev, const int64_t v_strides[3],
+                                int64_t window, int64_t sink_tokens, int64_t q_len,
+                                int64_t n_tokens, int batch, int q_heads, int kv_heads,
+                                int head_dim, int dtype, float scale, int num_splits,
+                                void* workspace_dev, size_t workspace_bytes,
+                                void* out_dev, const int64_t out_strides[3], void* stream);
+
+/* The same over page pools, as tc_prefill_paged_attention reads them. */
+int tc_prefill_paged_window_attention(const void* q_dev, const int64_t q_strides[3],
+                                      const void* k_pool_dev, const void* v_pool_dev,
+                                      const int64_t pool_strides[3], int num_pages,
+                                      const int32_t* tok_off_dev, int64_t tok_pitch,
+                                      int64_t window, int64_t sink_tokens, int64_t q_len,
+                                      int64_t n_tokens, int batch, int q_heads, int kv_heads,
+                                      int head_dim, int dtype, float scale, int num_splits,
+                                      void* workspace_dev, size_t workspace_bytes,
+                                      void* out_dev, const int64_t out_strides[3], void* stream);
+
+/* Key splits of a windowed call, or a negative TC_ERR_* code. */
+int tc_prefill_window_num_splits(int batch, int64_t q_len, int64_t n_tokens, int64_t window,
+                                 int64_t sink_tokens, int q_heads, int kv_heads);
 
 /* Key splits tc_prefill_attention uses with num_splits <= 0 (a negative value
  * is -TC_ERR_*): 1 for a prompt (at least half of the keys are the queries'

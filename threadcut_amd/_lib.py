@@ -76,6 +76,16 @@ SIGNATURES = {
     "tc_append_rows": (_I, [_P, _I64P, _P, _I64P, _P, _P, _I64P, _I64, _I64, _I, _I, _I64, _I, _I, _P]),
     "tc_paged_append_rows": (_I, [_PP, _I64P, _PP, _I64P, _PP, _PP, _I64P, _I, _I, _P, _I, _I, _I, _I64, _I, _I,
                                   _P]),
+    "tc_decode_window_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64, _I64, _I64, _I, _I, _I, _I, _I, _F,
+                                        _I, _P, _S, _P, _I64P, _P]),
+    "tc_decode_append_window_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64, _I64,
+                                               _I64, _I, _I, _I, _I, _I, _F, _I, _P, _S, _P, _I64P, _P]),
+    "tc_decode_window_tokens": (_I64, [_I64, _I64, _I64]),
+    "tc_prefill_window_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _I64, _I64, _I64, _I64, _I, _I, _I, _I, _I,
+                                         _F, _I, _P, _S, _P, _I64P, _P]),
+    "tc_prefill_paged_window_attention": (_I, [_P, _I64P, _P, _P, _I64P, _I, _P, _I64, _I64, _I64, _I64, _I64, _I, _I,
+                                               _I, _I, _I, _F, _I, _P, _S, _P, _I64P, _P]),
+    "tc_prefill_window_num_splits": (_I, [_I, _I64, _I64, _I64, _I64, _I, _I]),
     "tc_paged_append_rope": (_I, [_PP, _I64P, _PP, _I64P, _PP, _PP, _I64P, _I, _I, _P, _PP, _I64P, _PP, _I64P, _I, _FP,
                                   _P, _I, _I, _I, _I64, _I, _I, _P]),
     "tc_prefill_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _P, _S, _I, _I64, _I64, _I, _I,
@@ -212,6 +222,17 @@ def stream_of(device):
     torch.cuda.current_stream builds, about 2 us a call.)"""
     index = device.index
     return ctypes.c_void_p(raw_stream(torch.cuda.current_device() if index is None else index))
+
+
+def check_window(window, sink_tokens, n, what):
+    """The (window, sink tokens) of a sliding-window call over n tokens, or None where it hides nothing (no window)."""
+    if window is None:
+        if sink_tokens:
+            raise ValueError(f"{what}: sink_tokens need a window")
+        return None
+    if window < 1 or sink_tokens < 0:
+        raise ValueError(f"{what}: window {window} with {sink_tokens} sink tokens")
+    return None if n - window <= sink_tokens else (int(window), int(sink_tokens))
 
 
 def per_stream(copies, index, make):

@@ -40,15 +40,24 @@ def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=No
 
     query [b, hq, q, d] (usually a transposed view), key/value [b, hkv, n, d]
     (views into the cache). Returns ([b, q, hq, d] contiguous, None).
+
+    ``sliding_window`` (which transformers passes for its sliding layers) holds
+    where there is no mask: each query then sees the last `sliding_window` keys
+    up to its own and the first `sink_tokens` (default 0). A mask holds its own.
     """
+    window, sinks = kwargs.get("sliding_window"), kwargs.get("sink_tokens") or 0
+    if not window or attention_mask is not None:
+        window, sinks = None, 0
     b, hq, q, d = query.shape
     scaling = scaling if scaling is not None else query.shape[-1] ** -0.5
     layer = paged.layer_of(key)
     if layer is not None:  # a paged cache layer handed over its pools
-        return paged.attention(layer, query, attention_mask, scaling), None
+        return paged.attention(layer, query, attention_mask, scaling, window, sinks), None
     hkv = key.shape[1]
     g = hq // hkv
     pending = kv.take_pending(key)
+    if window is not None and (_lib.check_window(window, sinks, key.shape[2], NAME) or 1 < q < key.shape[2]):
+        return _windowed(query, key, value, pending, scaling, int(window), int(sinks)), None
     fast = _lib.FAST
     if q == 1 and attention_mask is None and fast is not None and query.is_cuda:
         # The whole call in native code; None for what it does not take (then as below).
@@ -93,6 +102,35 @@ def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=No
     out = F.scaled_dot_product_attention(query, repeat_kv(key, g), repeat_kv(value, g),
                                          attn_mask=attention_mask, scale=scaling, is_causal=is_causal)
     return out.transpose(1, 2).contiguous(), None
+
+
+def _windowed(query, key, value, pending, scaling, window, sinks):
+    """The call under a sliding window: the decode and prefill kernels where they take the tensors, else SDPA."""
+    b, hq, q, d = query.shape
+    hkv, n = key.shape[1], key.shape[2]
+    g = hq // hkv
+    if q == 1 and decode_supports(query, key, value):
+        out = torch.empty((b, 1, hq, d), dtype=query.dtype, device=query.device)
+        qg, og = query.reshape(b, hkv, g, d), out.view(b, hkv, g, d)
+        if pending is None:
+            decode_into(qg, key, value, scaling, og, window=window, sink_tokens=sinks)
+            return out
+        k_new, v_new = pending.pending
+        pending.pending = None
+        if pending.device_pos is not None:
+            decode_append_at(qg, pending.kbuf, pending.vbuf, k_new, v_new, pending.device_pos, scaling, og,
+                             window=window, sink_tokens=sinks)
+        else:
+            decode_append_into(qg, pending.kbuf, pending.vbuf, k_new, v_new, pending.n, scaling, og, window=window,
+                               sink_tokens=sinks)
+        return out
+    if pending is not None:
+        pending.flush()
+    if prefill.supports(query, key, None):
+        return prefill.prefill_attention(query, key, value, None, scaling, True, window=window, sink_tokens=sinks)
+    out = F.scaled_dot_product_attention(query, repeat_kv(key, g), repeat_kv(value, g), scale=scaling,
+                                         attn_mask=prefill.band_mask(q, n, window, sinks, query.device))
+    return out.transpose(1, 2).contiguous()
 
 
 AttentionInterface.register(NAME, attention)

@@ -124,6 +124,9 @@ struct PartialArgs {
   // into the head slab of the pools.
   const int32_t* tok_off;
   int64_t tok_pitch;
+  // Window (decode_partial_kernel<..., true>): sequence b's query sees its last
+  // `window` tokens, an appended one among them, and the first `sinks` ones.
+  int32_t window, sinks;
   // One split: the result itself, rounded to the element type as the combine
   // rounds it (null: the partial goes to o_part, lse_part).
   uint16_t* out;
@@ -280,8 +283,12 @@ constexpr float kLazyMax = 8.f;               // log2 units the running maximum 
 
 // APPEND: the kernel attends (and writes) the new token of an append call
 // (a.k_new != null); DIRECT: it writes the result (a.out != null), of one
-// split. The other instantiations carry none of that code.
-template <int DT, bool PAGED, bool APPEND, bool DIRECT, int W>
+// split. WINDOW (contiguous caches, tiles dealt round-robin): only the first
+// a.sinks tokens and the last a.window are read: the tokens between the two
+// are left out of the index space that the tiles are dealt from, in which the
+// window follows the sinks' last, perhaps partial, tile. The other
+// instantiations carry none of that code.
+template <int DT, bool PAGED, bool APPEND, bool DIRECT, int W, bool WINDOW = false>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? TC_DECODE_WPE_PAGED : TC_DECODE_WPE))) void decode_partial_kernel(const PartialArgs a) {
   using M = DecodeMma<DT>;
   using E = Elem<DT>;
@@ -370,6 +377,19 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? 
   } else if (a.lens) {
     len = min(max(a.longest_first ? len_b : a.lens[b], 0), len_cap);
   }
+  // The window's first token, and where it stands in the index space of the
+  // tiles (0: the sequence is read whole).
+  int32_t win0 = 0, win_at = 0;
+  const int32_t last = len;  // tokens in the cache
+  if constexpr (WINDOW) {
+    win0 = __builtin_amdgcn_readfirstlane(max(len + (APPEND ? 1 : 0) - a.window, 0));
+    if (win0 > a.sinks) {
+      win_at = (a.sinks + kWaveIter - 1) / kWaveIter * kWaveIter;
+      len = win_at + last - win0;
+    } else {
+      win0 = 0;
+    }
+  }
   const int32_t end = a.interleave ? len : min(tok + wave_tokens, len);
 
   // K: token n of the tile, bytes [64 i + 16 g, +16) for block i.
@@ -409,9 +429,19 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? 
       ++li;
       load_paged_tile(tl, kslab, vslab, row_k, row_v, a.sk_b * 2, a.sv_b * 2, a.pages, a.page_tokens, page, slot,
                       rows, koff, voff);
+    } else if constexpr (WINDOW) {
+      const bool sink = t0 < win_at;
+      const int32_t at = sink || t0 >= end ? t0 : t0 - win_at + win0;
+      load_tile(tl, kslab, vslab, row_k, row_v, t0 < end ? at : 0, t0 >= end ? 0 : sink ? a.sinks : last, koff, voff);
     } else {
       load_tile(tl, kslab, vslab, row_k, row_v, t0, end, koff, voff);
     }
+  };
+  // The index at which the keys of the tile at t0 end.
+  auto limit = [&](const Tile& tl, int32_t t0) -> int32_t {
+    if constexpr (PAGED) return t0 + tl.rows;
+    if constexpr (WINDOW) return t0 < win_at ? a.sinks : end;
+    return end;
   };
   Tile t[2];
   load(t[0], tok);
@@ -487,12 +517,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? 
     for (;;) {
       const int32_t tok1 = tok + tok_step, tok2 = tok1 + tok_step;
       load(t[1], tok1);
-      step(t[0], tok, PAGED ? tok + t[0].rows : end);
+      step(t[0], tok, limit(t[0], tok));
 #if TC_DECODE_STAMPS
       if (st_first == 0) st_first = __builtin_amdgcn_s_memrealtime();
 #endif
       load(t[0], tok2);
-      if (tok1 < end) step(t[1], tok1, PAGED ? tok1 + t[1].rows : end);
+      if (tok1 < end) step(t[1], tok1, limit(t[1], tok1));
       tok = tok2;
       if (tok >= end) break;
     }
@@ -540,7 +570,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? 
           }
         }
       } else {
-        dst = is_v ? a.v_w + b * a.sv_b + h * a.sv_h + len * a.sv_t : a.k_w + b * a.sk_b + h * a.sk_h + len * a.sk_t;
+        dst = is_v ? a.v_w + b * a.sv_b + h * a.sv_h + last * a.sv_t : a.k_w + b * a.sk_b + h * a.sk_h + last * a.sk_t;
       }
       if (dst) *reinterpret_cast<uint4*>(dst + chunk) = *reinterpret_cast<const uint4*>(src + chunk);
     }
@@ -779,18 +809,22 @@ int check_common(int batch, int kv_heads, int group, int head_dim, int dtype) {
 
 inline dim3 partial_grid(const PartialArgs& a, int batch) { return dim3(a.heads, a.splits, batch); }
 
-template <int DT, bool PAGED, bool APPEND, int W>
+template <int DT, bool PAGED, bool APPEND, int W, bool WINDOW = false>
 void launch_partial_waves(const PartialArgs& a, int batch, hipStream_t stream) {
   if (a.out)
-    hipLaunchKernelGGL((decode_partial_kernel<DT, PAGED, APPEND, true, W>), partial_grid(a, batch), dim3(64 * W), 0,
-                       stream, a);
+    hipLaunchKernelGGL((decode_partial_kernel<DT, PAGED, APPEND, true, W, WINDOW>), partial_grid(a, batch),
+                       dim3(64 * W), 0, stream, a);
   else
-    hipLaunchKernelGGL((decode_partial_kernel<DT, PAGED, APPEND, false, W>), partial_grid(a, batch), dim3(64 * W), 0,
-                       stream, a);
+    hipLaunchKernelGGL((decode_partial_kernel<DT, PAGED, APPEND, false, W, WINDOW>), partial_grid(a, batch),
+                       dim3(64 * W), 0, stream, a);
 }
 
 template <int DT, bool PAGED>
 void launch_partial_paged(const PartialArgs& a, int batch, int waves, hipStream_t stream) {
+  if constexpr (!PAGED) {
+    if (a.window && a.k_new) return launch_partial_waves<DT, false, true, kWaves, true>(a, batch, stream);
+    if (a.window) return launch_partial_waves<DT, false, false, kWaves, true>(a, batch, stream);
+  }
   if (a.k_new) return launch_partial_waves<DT, PAGED, true, kWaves>(a, batch, stream);
   if constexpr (!PAGED)
     if (waves == kShortWaves) return launch_partial_waves<DT, false, false, kShortWaves>(a, batch, stream);
@@ -920,12 +954,33 @@ struct Paged {
   int64_t tok_pitch = 0;
 };
 
+// The visible tokens of a windowed call: the last `window` and the first `sinks`.
+struct Window {
+  int64_t window, sinks;
+};
+
+// Index space that the tiles of the longest sequence of n_tokens span (PartialArgs::window).
+int64_t window_span(const Window& w, int64_t n_tokens) {
+  if (n_tokens - w.window <= w.sinks) return n_tokens;
+  return ceil_div(w.sinks, kWaveIter) * kWaveIter + w.window;
+}
+
+// *whole: the window hides nothing, so that the call is the plain one.
+int check_window(int64_t window, int64_t sinks, int64_t n_tokens, Window* w, bool* whole) {
+  if (n_tokens < 0 || window < 1 || sinks < 0)
+    return fail(TC_ERR_INVALID_ARGUMENT, "window %lld, %lld sink tokens of %lld", (long long)window, (long long)sinks,
+                (long long)n_tokens);
+  *w = Window{std::min(window, n_tokens), std::min(sinks, n_tokens)};
+  *whole = n_tokens - w->window <= w->sinks;
+  return TC_OK;
+}
+
 int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_dev, const int64_t k_strides[3],
                  const void* v_dev, const int64_t v_strides[3], const int32_t* lens_dev, int64_t n_tokens, int batch,
                  int kv_heads, int group, int head_dim, int dtype, float scale, int split_tokens, int num_splits,
                  float* o_part_dev, float* lse_part_dev, int interleave, const Append* app, void* stream,
                  const Paged* paged = nullptr, bool whole_call = false, void* out_dev = nullptr,
-                 const int64_t* out_strides = nullptr) {
+                 const int64_t* out_strides = nullptr, const Window* window = nullptr) {
   int rc = check_common(batch, kv_heads, group, head_dim, dtype);
   if (rc != TC_OK) return rc;
   if (n_tokens == 0 && num_splits == 0) return TC_OK;  // empty caches: nothing to read
@@ -944,7 +999,7 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
                 kSplitGranule);
   if (num_splits < 0 || num_splits > TC_MAX_SPLITS)
     return fail(TC_ERR_INVALID_ARGUMENT, "num_splits %d outside [0, %d]", num_splits, TC_MAX_SPLITS);
-  if (static_cast<int64_t>(num_splits) * split_tokens < n_tokens)
+  if (static_cast<int64_t>(num_splits) * split_tokens < (window ? window_span(*window, n_tokens) : n_tokens))
     return fail(TC_ERR_INVALID_ARGUMENT, "%d splits of %d tokens do not cover %lld tokens", num_splits, split_tokens,
                 (long long)n_tokens);
   if (static_cast<int64_t>(num_splits) * split_tokens > 2 * kMaxTokens)
@@ -994,6 +1049,8 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
   a.page_tokens = paged ? paged->page_tokens : 0;
   a.tok_off = paged ? paged->tok_off : nullptr;
   a.tok_pitch = paged ? paged->tok_pitch : 0;
+  a.window = window ? static_cast<int32_t>(window->window) : 0;
+  a.sinks = window ? static_cast<int32_t>(window->sinks) : 0;
   a.out = static_cast<uint16_t*>(out_dev);
   a.so_b = out_dev ? out_strides[0] : 0;
   a.so_h = out_dev ? out_strides[1] : 0;
@@ -1078,12 +1135,14 @@ int attention_impl(const void* q_dev, const int64_t q_strides[3], const void* k_
                    const void* v_dev, const int64_t v_strides[3], const int32_t* lens_dev, int64_t n_tokens,
                    int batch, int kv_heads, int group, int head_dim, int dtype, float scale, int split_tokens,
                    void* workspace_dev, size_t workspace_bytes, void* out_dev, const int64_t out_strides[3],
-                   const Append* app, int ragged_plan, void* stream, const Paged* paged = nullptr) {
+                   const Append* app, int ragged_plan, void* stream, const Paged* paged = nullptr,
+                   const Window* window = nullptr) {
   int rc = check_common(batch, kv_heads, group, head_dim, dtype);
   if (rc != TC_OK) return rc;
   if (n_tokens < 0) return fail(TC_ERR_INVALID_ARGUMENT, "n_tokens %lld is negative", (long long)n_tokens);
   int S = 0, t = 0;
-  if ((rc = split_plan(batch, kv_heads, n_tokens, split_tokens, ragged_plan, &S, &t)) != TC_OK) return rc;
+  const int64_t span = window ? window_span(*window, n_tokens) : n_tokens;
+  if ((rc = split_plan(batch, kv_heads, span, split_tokens, ragged_plan, &S, &t)) != TC_OK) return rc;
   const size_t need = tc_decode_workspace_bytes(batch, kv_heads, group, head_dim, S);
   if (S > 0 && (!workspace_dev || workspace_bytes < need))
     return fail(TC_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed for %d splits", workspace_bytes, need, S);
@@ -1102,7 +1161,7 @@ int attention_impl(const void* q_dev, const int64_t q_strides[3], const void* k_
     // Splits here are internal, so their tiles are dealt round-robin (the merged result is the same).
     rc = partial_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch, kv_heads, group,
                       head_dim, dtype, scale, t, S, o_part, lse_part, TC_DECODE_INTERLEAVE, app, stream, paged,
-                      true, direct ? out_dev : nullptr, out_strides);
+                      true, direct ? out_dev : nullptr, out_strides, window);
     if (rc != TC_OK || direct) return rc;
   }
   return tc_decode_combine(o_part, lse_part, batch, kv_heads, group, head_dim, S, out_dev, out_strides, dtype, stream);
@@ -1122,6 +1181,34 @@ int tc_decode_attention(const void* q_dev, const int64_t q_strides[3], const voi
   return attention_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch, kv_heads,
                         group, head_dim, dtype, scale, split_tokens, workspace_dev, workspace_bytes, out_dev,
                         out_strides, nullptr, lens_dev != nullptr, stream);
+}
+
+}  // extern "C"
+
+extern "C" {
+
+int64_t tc_decode_window_tokens(int64_t n_tokens, int64_t window, int64_t sink_tokens) {
+  clear_error();
+  Window w;
+  bool whole;
+  const int rc = check_window(window, sink_tokens, n_tokens, &w, &whole);
+  return rc == TC_OK ? window_span(w, n_tokens) : -rc;
+}
+
+int tc_decode_window_attention(const void* q_dev, const int64_t q_strides[3], const void* k_dev,
+                               const int64_t k_strides[3], const void* v_dev, const int64_t v_strides[3],
+                               const int32_t* lens_dev, int64_t n_tokens, int64_t window, int64_t sink_tokens,
+                               int batch, int kv_heads, int group, int head_dim, int dtype, float scale,
+                               int split_tokens, void* workspace_dev, size_t workspace_bytes, void* out_dev,
+                               const int64_t out_strides[3], void* stream) {
+  clear_error();
+  Window w;
+  bool whole;
+  const int rc = check_window(window, sink_tokens, n_tokens, &w, &whole);
+  if (rc != TC_OK) return rc;
+  return attention_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch, kv_heads,
+                        group, head_dim, dtype, scale, split_tokens, workspace_dev, workspace_bytes, out_dev,
+                        out_strides, nullptr, lens_dev != nullptr, stream, nullptr, whole ? nullptr : &w);
 }
 
 }  // extern "C"
@@ -1195,7 +1282,7 @@ static int append_impl(const void* q_dev, const int64_t q_strides[3], void* k_ca
                        const int64_t k_new_strides[2], const void* v_new_dev, const int64_t v_new_strides[2],
                        const int32_t* pos_dev, int64_t n_tokens, int batch, int kv_heads, int group, int head_dim,
                        int dtype, float scale, int split_tokens, void* workspace_dev, size_t workspace_bytes,
-                       void* out_dev, const int64_t out_strides[3], void* stream) {
+                       void* out_dev, const int64_t out_strides[3], void* stream, const Window* window = nullptr) {
   if (n_tokens < 1) return fail(TC_ERR_INVALID_ARGUMENT, "append needs n_tokens >= 1 (got %lld)", (long long)n_tokens);
   if (!k_new_dev || !v_new_dev || !k_new_strides || !v_new_strides)
     return fail(TC_ERR_INVALID_ARGUMENT, "null new-token K/V");
@@ -1207,7 +1294,7 @@ static int append_impl(const void* q_dev, const int64_t q_strides[3], void* k_ca
   const Append app{k_new_dev, k_new_strides, v_new_dev, v_new_strides, k_cache_dev, v_cache_dev};
   return attention_impl(q_dev, q_strides, k_cache_dev, k_strides, v_cache_dev, v_strides, pos_dev, n_tokens, batch,
                         kv_heads, group, head_dim, dtype, scale, split_tokens, workspace_dev, workspace_bytes, out_dev,
-                        out_strides, &app, 0, stream);
+                        out_strides, &app, 0, stream, nullptr, window);
 }
 
 int tc_decode_append_attention(const void* q_dev, const int64_t q_strides[3], void* k_cache_dev,
@@ -1234,6 +1321,24 @@ int tc_decode_append_attention_at(const void* q_dev, const int64_t q_strides[3],
   return append_impl(q_dev, q_strides, k_cache_dev, k_strides, v_cache_dev, v_strides, k_new_dev, k_new_strides,
                      v_new_dev, v_new_strides, pos_dev, capacity, batch, kv_heads, group, head_dim, dtype, scale,
                      split_tokens, workspace_dev, workspace_bytes, out_dev, out_strides, stream);
+}
+
+int tc_decode_append_window_attention(const void* q_dev, const int64_t q_strides[3], void* k_cache_dev,
+                                      const int64_t k_strides[3], void* v_cache_dev, const int64_t v_strides[3],
+                                      const void* k_new_dev, const int64_t k_new_strides[2], const void* v_new_dev,
+                                      const int64_t v_new_strides[2], const int32_t* pos_dev, int64_t n_tokens,
+                                      int64_t window, int64_t sink_tokens, int batch, int kv_heads, int group,
+                                      int head_dim, int dtype, float scale, int split_tokens, void* workspace_dev,
+                                      size_t workspace_bytes, void* out_dev, const int64_t out_strides[3],
+                                      void* stream) {
+  clear_error();
+  Window w;
+  bool whole;
+  const int rc = check_window(window, sink_tokens, n_tokens, &w, &whole);
+  if (rc != TC_OK) return rc;
+  return append_impl(q_dev, q_strides, k_cache_dev, k_strides, v_cache_dev, v_strides, k_new_dev, k_new_strides,
+                     v_new_dev, v_new_strides, pos_dev, n_tokens, batch, kv_heads, group, head_dim, dtype, scale,
+                     split_tokens, workspace_dev, workspace_bytes, out_dev, out_strides, stream, whole ? nullptr : &w);
 }
 
 int tc_decode_paged_attention(const void* q_dev, const int64_t q_strides[3], const void* k_pool_dev,

@@ -90,6 +90,7 @@ struct PrefillArgs {
   int mask_words;           // mask rows 4-byte aligned: a tile's mask bytes load as words
   int whole;                // contiguous K/V: (n + 128) rows of each fit 31 bits (one buffer range a slab)
   int fold_cus;             // > 0: pair work items w and W-1-w on one CU (see the kernel), W <= 2 x this
+  int32_t window, sinks;    // windowed kernels: a row sees the last `window` keys up to its own and the first `sinks`
   float c;                  // |scale| * log2(e), > 0 (neg: 1 for a negative scale, -1 for scale 0)
   // Paged K/V (prefill_kernel<DT, G, true>): k and v are page pools whose head
   // slabs start at k + h * sk_h (v + h * sv_h); the row of sequence b's
@@ -188,7 +189,11 @@ struct Shape {
   static constexpr int kTileKeys = kWaveKeys * KEYGROUPS;
 };
 
-template <int DT, int G, bool PAGED, class S>
+// WINDOW: causal rows that see only the last a.window keys up to their own and
+// the first a.sinks. Tile indices then count the tiles that a work-group may
+// need: those of the sinks, and from the first key that its first row's window
+// holds on; `skip` tiles between the two are left out.
+template <int DT, int G, bool PAGED, class S, bool WINDOW = false>
 __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(TC_PREFILL_WAVES, TC_PREFILL_WAVES))) void prefill_kernel(
     const PrefillArgs a) {
   constexpr int kTileKeys = S::kTileKeys;
@@ -359,7 +364,14 @@ __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(
   const int32_t key_end = a.causal ? min(n32, past + last_tok + 1) : n32;
   const int32_t split_tiles = static_cast<int32_t>(a.split_tiles);
   const int32_t t_begin = split * split_tiles;
-  const int32_t nt = min((key_end + kTileKeys - 1) / kTileKeys, t_begin + split_tiles);
+  int32_t skip_at = 0, skip = 0;
+  if constexpr (WINDOW) {
+    const int32_t first_tile = max(past + tok0 - a.window + 1, 0) / kTileKeys;
+    skip_at = (a.sinks + kTileKeys - 1) / kTileKeys;
+    skip = max(first_tile - skip_at, 0);
+  }
+  auto at = [&](int32_t tile) -> int32_t { return WINDOW && tile >= skip_at ? tile + skip : tile; };
+  const int32_t nt = min((key_end + kTileKeys - 1) / kTileKeys - skip, t_begin + split_tiles);
   // The classes of a window of 64 tiles from `base` on, one bit a tile: lane i
   // works out tile base + i, and ballots leave the window in scalar registers,
   // so that finding the next active tile and its class takes a shift and a
@@ -379,18 +391,22 @@ __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(
   auto window = [&](int32_t first) {
     base = first;
     const int32_t tile = first + lane;
-    const int32_t key0 = tile * kTileKeys + kg * S::kWaveKeys;
+    const int32_t key0 = at(tile) * kTileKeys + kg * S::kWaveKeys;
     const bool on = tile < nt;
     bool some = on;
     int c = TILE_MIXED;
-    if (tcls) {
+    if constexpr (WINDOW) {
+      const int32_t key1 = key0 + S::kWaveKeys - 1, low = past + tok0, high = past + last_tok;
+      c = key0 <= high && (key1 > low - a.window || key0 < a.sinks) ? TILE_CAUSAL : TILE_SKIP;
+      if (key1 <= low && (key0 > high - a.window || key1 < a.sinks)) c = TILE_FULL;
+    } else if (tcls) {
       some = map_next != 0;
       c = static_cast<int>(kMapTiles == 1 ? map_next : (map_next >> (8 * (key0 / kKeys % kMapTiles))) & 0xffu);
       map_next = map_load(tile + 64);
     } else if (!a.mask && key0 + S::kWaveKeys <= n32) {
       c = a.causal ? TILE_CAUSAL : TILE_FULL;
     }
-    if (c == TILE_CAUSAL && (S::kKeyGroups > 1 || !tcls)) {
+    if (!WINDOW && c == TILE_CAUSAL && (S::kKeyGroups > 1 || !tcls)) {
       c = key0 + S::kWaveKeys - 1 > past + tok0 ? TILE_CAUSAL : TILE_FULL;
       if (S::kKeyGroups > 1 && key0 > past + last_tok) c = TILE_SKIP;
     }
@@ -449,10 +465,10 @@ __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(
   auto load_first = [&](int32_t tile) {
     int32_t rows_t = kNoRow, first_t = -1;
     if constexpr (PAGED) {
-      rows_t = tile_rows(tile);
+      rows_t = tile_rows(at(tile));
       first_t = contiguous_from(rows_t);
     }
-    dma_tile(s_k0, s_v0, tile, rows_t, first_t);
+    dma_tile(s_k0, s_v0, at(tile), rows_t, first_t);
   };
   if (t_begin < nt) load_first(t_begin);
   // Q^T as the MFMA B operand: dims 16c + 8*hi .. +8 of the lane's row, loaded
@@ -493,7 +509,7 @@ __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(
   }
   // Paged: the row offsets of the tile loaded next, fetched one tile ahead.
   int32_t rows_n = kNoRow;
-  if constexpr (PAGED) rows_n = tn < nt ? tile_rows(tn) : kNoRow;
+  if constexpr (PAGED) rows_n = tn < nt ? tile_rows(at(tn)) : kNoRow;
   __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 
@@ -559,7 +575,7 @@ __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(
     {
       // Hidden keys of this lane's row (none on a FULL tile) score -inf, and
       // their exponentials are 0. Key 32 kt + 8 q + 4 hi + j of the wave's.
-      const int32_t key0 = t * kTileKeys + kg * S::kWaveKeys;
+      const int32_t key0 = at(t) * kTileKeys + kg * S::kWaveKeys;
       if (cls == TILE_MIXED && a.mask) {
         // By the row's mask bytes, read as one batch of loads (one wait, no
         // branch per key): aligned words (word q of half kt at byte
@@ -593,10 +609,22 @@ __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(
         // By position: from the row's own key on (causal), or from n on.
         int32_t lim = n32 - key0 - 4 * hi;
         if (a.causal || cls == TILE_CAUSAL) lim = min(lim, past + tok + 1 - key0 - 4 * hi);
+        if constexpr (WINDOW) {
+          // The row's window begins at key `low` of the wave's, the sinks end at `sink`.
+          const int32_t own = past + tok - key0 - 4 * hi, low = own - a.window + 1, sink = a.sinks - key0 - 4 * hi;
 #pragma unroll
-        for (int kt = 0; kt < kHalves; ++kt)
+          for (int kt = 0; kt < kHalves; ++kt)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) s[kt][v] = 32 * kt + acc_key(v, 0) < lim ? s[kt][v] : neg_inf();
+            for (int v = 0; v < 16; ++v) {
+              const int32_t k = 32 * kt + acc_key(v, 0);
+              s[kt][v] = (k < lim) & ((k >= low) | (k < sink)) ? s[kt][v] : neg_inf();
+            }
+        } else {
+#pragma unroll
+          for (int kt = 0; kt < kHalves; ++kt)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[kt][v] = 32 * kt + acc_key(v, 0) < lim ? s[kt][v] : neg_inf();
+        }
       }
       // Four independent max chains (fmax is exact in any order).
       float m4[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
@@ -686,13 +714,13 @@ __global__ __launch_bounds__(64 * S::kWaves) __attribute__((amdgpu_waves_per_eu(
     if constexpr (PAGED) first_tn = more ? contiguous_from(rows_tn) : -1;
     int cls_nn = TILE_SKIP;
     const int32_t tnn = next_active(tn + 1, cls_nn);
-    if constexpr (PAGED) rows_n = tnn < nt ? tile_rows(tnn) : kNoRow;
+    if constexpr (PAGED) rows_n = tnn < nt ? tile_rows(at(tnn)) : kNoRow;
     const int cls = cls_t;
 
     // The next tile's loads go out first, in one burst: spread between the
     // MFMAs below they stall the MFMA issue.
     if (more) {
-      dma_tile(dk, dv, tn, rows_tn, first_tn);
+      dma_tile(dk, dv, at(tn), rows_tn, first_tn);
     }
     // With several key groups a wave's own keys may all be hidden.
     if (S::kKeyGroups == 1 || cls != TILE_SKIP) attend(lk, lv, cls);
@@ -1022,7 +1050,7 @@ typedef Shape<2, 4, 1> Deep;    // 64 rows, 128-key tiles, 8 waves: one work-gro
 typedef Shape<2, 2, 1> Narrow;  // 64 rows, 64-key tiles, 4 waves: two work-groups a CU
 enum : int { SHAPE_WIDE = 0, SHAPE_TALL = 1, SHAPE_DEEP = 2, SHAPE_NARROW = 3 };
 
-template <int DT, bool PAGED, class S>
+template <int DT, bool PAGED, class S, bool WINDOW = false>
 void launch_attention(const PrefillArgs& a_in, int group, dim3 grid, hipStream_t stream) {
   PrefillArgs a = a_in;
 #if TC_PREFILL_STAMPS
@@ -1030,16 +1058,20 @@ void launch_attention(const PrefillArgs& a_in, int group, dim3 grid, hipStream_t
 #endif
   const dim3 block(64 * S::kWaves);
   switch (group) {
-    case 1: hipLaunchKernelGGL((prefill_kernel<DT, 1, PAGED, S>), grid, block, 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((prefill_kernel<DT, 2, PAGED, S>), grid, block, 0, stream, a); break;
-    case 4: hipLaunchKernelGGL((prefill_kernel<DT, 4, PAGED, S>), grid, block, 0, stream, a); break;
-    default: hipLaunchKernelGGL((prefill_kernel<DT, 8, PAGED, S>), grid, block, 0, stream, a); break;
+    case 1: hipLaunchKernelGGL((prefill_kernel<DT, 1, PAGED, S, WINDOW>), grid, block, 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((prefill_kernel<DT, 2, PAGED, S, WINDOW>), grid, block, 0, stream, a); break;
+    case 4: hipLaunchKernelGGL((prefill_kernel<DT, 4, PAGED, S, WINDOW>), grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL((prefill_kernel<DT, 8, PAGED, S, WINDOW>), grid, block, 0, stream, a); break;
   }
 }
 
 template <int DT, class S>
 void launch_shape(const PrefillArgs& a, int group, dim3 grid, hipStream_t stream) {
-  if (a.tok_off)
+  if (a.window && a.tok_off)
+    launch_attention<DT, true, S, true>(a, group, grid, stream);
+  else if (a.window)
+    launch_attention<DT, false, S, true>(a, group, grid, stream);
+  else if (a.tok_off)
     launch_attention<DT, true, S>(a, group, grid, stream);
   else
     launch_attention<DT, false, S>(a, group, grid, stream);
@@ -1195,6 +1227,21 @@ int plan(int batch, int64_t q_len, int64_t n, int group, int kv_heads, int reque
   return TC_OK;
 }
 
+// The window of a call whose rows see the last `window` keys up to their own and the first `sinks`.
+struct Window {
+  int64_t window, sinks;
+};
+
+// Keys that a work-group of a windowed call may walk, at most, which is what the plan goes by in place of all n: the
+// sinks and the windows of its rows, in whole tiles.
+int64_t window_keys(const Window& w, int64_t n, int group) {
+  const int64_t most = ceil_div(std::min(w.sinks, n), 2 * kKeys) * 2 * kKeys + std::min(w.window, n) + 128 / group + 2 * kKeys;
+  return std::min(n, most);
+}
+
+// True where the window hides nothing from anybody.
+bool window_open(const Window& w, int64_t n) { return w.window >= n || n - w.window <= w.sinks; }
+
 size_t workspace_bytes(int batch, int64_t q_len, int q_heads, int splits) {
   if (splits <= 1) return 0;
   return static_cast<size_t>(batch) * splits * q_len * q_heads * (kHeadDim + 1) * sizeof(float);
@@ -1212,6 +1259,21 @@ extern "C" int tc_prefill_num_splits(int batch, int64_t q_len, int64_t n_tokens,
   if ((rc = check_group(q_heads, kv_heads, &group)) != TC_OK) return -rc;
   Plan p;
   if ((rc = plan(batch, q_len, n_tokens, group, kv_heads, 0, true, false, &p)) != TC_OK) return -rc;
+  return p.splits;
+}
+
+extern "C" int tc_prefill_window_num_splits(int batch, int64_t q_len, int64_t n_tokens, int64_t window,
+                                            int64_t sink_tokens, int q_heads, int kv_heads) {
+  clear_error();
+  int group = 0, rc;
+  if (batch < 1 || q_len < 0 || n_tokens < q_len || window < 1 || sink_tokens < 0)
+    return -fail(TC_ERR_INVALID_ARGUMENT, "batch %d, q_len %lld, n %lld, window %lld, %lld sink tokens", batch,
+                 (long long)q_len, (long long)n_tokens, (long long)window, (long long)sink_tokens);
+  if ((rc = check_group(q_heads, kv_heads, &group)) != TC_OK) return -rc;
+  const Window w{window, sink_tokens};
+  Plan p;
+  if ((rc = plan(batch, q_len, window_open(w, n_tokens) ? n_tokens : window_keys(w, n_tokens, group), group, kv_heads, 0,
+                 true, false, &p)) != TC_OK) return -rc;
   return p.splits;
 }
 
@@ -1277,8 +1339,12 @@ int prefill_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
                  const int64_t mask_strides[3], const uint8_t* mask_tiles_dev, size_t mask_tiles_bytes, int causal,
                  int64_t q_len, int64_t n_tokens, int batch, int q_heads, int kv_heads, int head_dim, int dtype,
                  float scale, int num_splits, void* workspace_dev, size_t workspace_bytes_in, void* out_dev,
-                 const int64_t out_strides[3], void* stream, const PagedPools* pools) {
+                 const int64_t out_strides[3], void* stream, const PagedPools* pools, const Window* window = nullptr) {
   int group = 0, rc;
+  if (window && (window->window < 1 || window->sinks < 0))
+    return fail(TC_ERR_INVALID_ARGUMENT, "window %lld, %lld sink tokens", (long long)window->window,
+                (long long)window->sinks);
+  if (window && window_open(*window, n_tokens)) window = nullptr;
   if (batch < 1 || batch > 65535) return fail(TC_ERR_INVALID_ARGUMENT, "batch %d", batch);
   if ((rc = check_group(q_heads, kv_heads, &group)) != TC_OK) return rc;
   if (head_dim != kHeadDim) return fail(TC_ERR_UNSUPPORTED, "head_dim %d unsupported (kernels are built for 128)", head_dim);
@@ -1324,8 +1390,8 @@ int prefill_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
   // One 32-bit buffer range over a head's slab, with room for the tiles' rows past n.
   const bool whole = !pools && (n_tokens + 2 * kKeys) * 2 * std::max(k_strides[2], v_strides[2]) < (int64_t(1) << 31);
   Plan p;
-  if ((rc = plan(batch, q_len, n_tokens, group, kv_heads, num_splits, pools || whole, !causal && !mask_dev,
-                 &p)) != TC_OK) return rc;
+  if ((rc = plan(batch, q_len, window ? window_keys(*window, n_tokens, group) : n_tokens, group, kv_heads, num_splits,
+                 pools || whole, !causal && !mask_dev, &p)) != TC_OK) return rc;
   const int splits = p.splits;
   if (p.nblk * kv_heads * batch * splits > 0x7fffffff) return fail(TC_ERR_UNSUPPORTED, "grid too large");
   const size_t need = workspace_bytes(batch, q_len, q_heads, splits);
@@ -1354,6 +1420,8 @@ int prefill_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
   a.mask_words = mask_dev && reinterpret_cast<uintptr_t>(mask_dev) % 4 == 0 && a.sm_b % 4 == 0 && a.sm_q % 4 == 0;
   a.whole = whole;
   a.so_b = out_strides[0]; a.so_t = out_strides[1]; a.so_h = out_strides[2];
+  a.window = window ? static_cast<int32_t>(window->window) : 0;
+  a.sinks = window ? static_cast<int32_t>(std::min(window->sinks, n_tokens)) : 0;
   a.q_len = q_len;
   a.n = n_tokens;
   a.nblk = p.nblk;
@@ -1408,15 +1476,12 @@ extern "C" int tc_prefill_attention(const void* q_dev, const int64_t q_strides[3
                       num_splits, workspace_dev, workspace_bytes_in, out_dev, out_strides, stream, nullptr);
 }
 
-extern "C" int tc_prefill_paged_attention(const void* q_dev, const int64_t q_strides[3], const void* k_pool_dev,
-                                          const void* v_pool_dev, const int64_t pool_strides[3], int num_pages,
-                                          const int32_t* tok_off_dev, int64_t tok_pitch, const uint8_t* mask_dev,
-                                          const int64_t mask_strides[3], const uint8_t* mask_tiles_dev,
-                                          size_t mask_tiles_bytes, int causal, int64_t q_len, int64_t n_tokens,
-                                          int batch, int q_heads, int kv_heads, int head_dim, int dtype, float scale,
-                                          int num_splits, void* workspace_dev, size_t workspace_bytes_in,
-                                          void* out_dev, const int64_t out_strides[3], void* stream) {
-  clear_error();
+namespace tc {
+namespace {
+
+// The pools of a paged call, checked.
+int paged_pools(const int64_t* pool_strides, int num_pages, const int32_t* tok_off_dev, int64_t tok_pitch, int64_t q_len,
+                int64_t n_tokens, int kv_heads, PagedPools* out) {
   if (!pool_strides) return fail(TC_ERR_INVALID_ARGUMENT, "null pool strides");
   if (num_pages < 1) return fail(TC_ERR_INVALID_ARGUMENT, "pool of %d pages", num_pages);
   if (q_len > 0 && (!tok_off_dev || tok_pitch < n_tokens))
@@ -1429,11 +1494,59 @@ extern "C" int tc_prefill_paged_attention(const void* q_dev, const int64_t q_str
       static_cast<int64_t>(kv_heads - 1) * pool_strides[1] * 2 >= pool_bytes)
     return fail(TC_ERR_UNSUPPORTED, "pool of %lld bytes (page stride %lld): paged prefill needs a pool under 2 GiB",
                 (long long)pool_bytes, (long long)pool_strides[0]);
-  const PagedPools pools{tok_off_dev, tok_pitch, pool_bytes};
+  *out = PagedPools{tok_off_dev, tok_pitch, pool_bytes};
+  return TC_OK;
+}
+
+}  // namespace
+}  // namespace tc
+
+extern "C" int tc_prefill_paged_attention(const void* q_dev, const int64_t q_strides[3], const void* k_pool_dev,
+                                          const void* v_pool_dev, const int64_t pool_strides[3], int num_pages,
+                                          const int32_t* tok_off_dev, int64_t tok_pitch, const uint8_t* mask_dev,
+                                          const int64_t mask_strides[3], const uint8_t* mask_tiles_dev,
+                                          size_t mask_tiles_bytes, int causal, int64_t q_len, int64_t n_tokens,
+                                          int batch, int q_heads, int kv_heads, int head_dim, int dtype, float scale,
+                                          int num_splits, void* workspace_dev, size_t workspace_bytes_in,
+                                          void* out_dev, const int64_t out_strides[3], void* stream) {
+  clear_error();
+  PagedPools pools;
+  const int rc = paged_pools(pool_strides, num_pages, tok_off_dev, tok_pitch, q_len, n_tokens, kv_heads, &pools);
+  if (rc != TC_OK) return rc;
   return prefill_impl(q_dev, q_strides, k_pool_dev, pool_strides, v_pool_dev, pool_strides, mask_dev, mask_strides,
                       mask_tiles_dev, mask_tiles_bytes, causal, q_len, n_tokens, batch, q_heads, kv_heads, head_dim,
                       dtype, scale, num_splits, workspace_dev, workspace_bytes_in, out_dev, out_strides, stream,
                       &pools);
+}
+
+extern "C" int tc_prefill_window_attention(const void* q_dev, const int64_t q_strides[3], const void* k_dev,
+                                           const int64_t k_strides[3], const void* v_dev, const int64_t v_strides[3],
+                                           int64_t window, int64_t sink_tokens, int64_t q_len, int64_t n_tokens,
+                                           int batch, int q_heads, int kv_heads, int head_dim, int dtype, float scale,
+                                           int num_splits, void* workspace_dev, size_t workspace_bytes_in,
+                                           void* out_dev, const int64_t out_strides[3], void* stream) {
+  clear_error();
+  const Window w{window, sink_tokens};
+  return prefill_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, nullptr, nullptr, nullptr, 0, 1, q_len,
+                      n_tokens, batch, q_heads, kv_heads, head_dim, dtype, scale, num_splits, workspace_dev,
+                      workspace_bytes_in, out_dev, out_strides, stream, nullptr, &w);
+}
+
+extern "C" int tc_prefill_paged_window_attention(const void* q_dev, const int64_t q_strides[3], const void* k_pool_dev,
+                                                 const void* v_pool_dev, const int64_t pool_strides[3], int num_pages,
+                                                 const int32_t* tok_off_dev, int64_t tok_pitch, int64_t window,
+                                                 int64_t sink_tokens, int64_t q_len, int64_t n_tokens, int batch,
+                                                 int q_heads, int kv_heads, int head_dim, int dtype, float scale,
+                                                 int num_splits, void* workspace_dev, size_t workspace_bytes_in,
+                                                 void* out_dev, const int64_t out_strides[3], void* stream) {
+  clear_error();
+  PagedPools pools;
+  const int rc = paged_pools(pool_strides, num_pages, tok_off_dev, tok_pitch, q_len, n_tokens, kv_heads, &pools);
+  if (rc != TC_OK) return rc;
+  const Window w{window, sink_tokens};
+  return prefill_impl(q_dev, q_strides, k_pool_dev, pool_strides, v_pool_dev, pool_strides, nullptr, nullptr, nullptr, 0,
+                      1, q_len, n_tokens, batch, q_heads, kv_heads, head_dim, dtype, scale, num_splits, workspace_dev,
+                      workspace_bytes_in, out_dev, out_strides, stream, &pools, &w);
 }
 
 #if TC_PREFILL_STAMPS

@@ -93,6 +93,14 @@ def _plan(device_index, b, hkv, g, d, n, split, ragged):
     return s, max(lib.tc_decode_workspace_bytes(b, hkv, g, d, s), 16)
 
 
+def _window_tokens(n, window, sink_tokens):
+    """Tokens that a windowed call's split plan is made for."""
+    t = _lib.load().tc_decode_window_tokens(n, window, sink_tokens)
+    if t < 0:
+        _lib.check(-t, "tc_decode_window_tokens")
+    return t
+
+
 def _on_device(device):
     """Context that makes `device` current, or nothing when it already is (the common case)."""
     if device.index is None or device.index == torch.cuda.current_device():
@@ -111,13 +119,14 @@ class _NoSwitch:
 _NO_SWITCH = _NoSwitch()
 
 
-def decode_into(q, k, v, scale, out, lens=None, split=None):
+def decode_into(q, k, v, scale, out, lens=None, split=None, window=None, sink_tokens=0):
     """out[b,h,g,:] = softmax(q[b,h,g]·k[b,h,:len_b]ᵀ·scale)·v[b,h,:len_b] (fp32 math).
 
     q [B,Hkv,G,D], k/v [B,Hkv,N,D] (any strides, last dim contiguous), out
     [B,Hkv,G,D] in q.dtype, lens optional int32 [B] on the device (every
-    lens[b] <= N; without lens all N tokens are used). Enqueued on the
-    current stream; returns out.
+    lens[b] <= N; without lens all N tokens are used). With a ``window`` only
+    the last `window` of a sequence's tokens and its first `sink_tokens` are
+    attended (and read). Enqueued on the current stream; returns out.
     """
     _check_qkv(q, k, v, "decode_attention")
     b, hkv, g, d = q.shape
@@ -129,9 +138,18 @@ def decode_into(q, k, v, scale, out, lens=None, split=None):
             raise ValueError("decode_attention: lens must be a contiguous int32 [B] tensor on the device")
     lib = _lib.load()
     dt = _lib.dtype_code(q.dtype)
-    _, nbytes = _plan(q.device.index, b, hkv, g, d, n, split, lens is not None)
+    w = _lib.check_window(window, sink_tokens, n, "decode_attention")
+    _, nbytes = _plan(q.device.index, b, hkv, g, d, n if w is None else _window_tokens(n, *w), split, lens is not None)
     with _on_device(q.device):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        if w is not None:
+            rc = lib.tc_decode_window_attention(
+                q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k, True), v.data_ptr(), _strides3(v, True),
+                lens.data_ptr() if lens is not None else None, n, *w,
+                b, hkv, g, d, dt, float(scale), int(split or 0),
+                ws.data_ptr(), ws.numel(), out.data_ptr(), _strides3(out), _lib.stream_of(q.device))
+            _lib.check(rc, "tc_decode_window_attention")
+            return out
         rc = lib.tc_decode_attention(
             q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k, True), v.data_ptr(), _strides3(v, True),
             lens.data_ptr() if lens is not None else None, n,
@@ -141,12 +159,39 @@ def decode_into(q, k, v, scale, out, lens=None, split=None):
     return out
 
 
-def decode_append_into(q, k_cache, v_cache, k_new, v_new, n, scale, out, split=None):
+def _append(q, k_cache, v_cache, kn, vn, pos, n, scale, out, split, window, sink_tokens, what):
+    """The library call of decode_append_into and decode_append_at (pos: a tensor), of checked tensors."""
+    b, hkv, g, d = q.shape
+    lib = _lib.load()
+    w = _lib.check_window(window, sink_tokens, n, what)
+    _, nbytes = _plan(q.device.index, b, hkv, g, d, n if w is None else _window_tokens(n, *w), split, False)
+    with _on_device(q.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        st2 = lambda t: _lib.i64x2(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+        args = (q.data_ptr(), _strides3(q), k_cache.data_ptr(), _strides3(k_cache, True), v_cache.data_ptr(),
+                _strides3(v_cache, True), kn.data_ptr(), st2(kn), vn.data_ptr(), st2(vn))
+        rest = (b, hkv, g, d, _lib.dtype_code(q.dtype), float(scale), int(split or 0),
+                ws.data_ptr(), ws.numel(), out.data_ptr(), _strides3(out), _lib.stream_of(q.device))
+        if w is not None:
+            name = "tc_decode_append_window_attention"
+            rc = lib.tc_decode_append_window_attention(*args, None if pos is None else pos.data_ptr(), n, *w, *rest)
+        elif pos is not None:
+            name = "tc_decode_append_attention_at"
+            rc = lib.tc_decode_append_attention_at(*args, pos.data_ptr(), n, *rest)
+        else:
+            name = "tc_decode_append_attention"
+            rc = lib.tc_decode_append_attention(*args, n, *rest)
+        _lib.check(rc, name)
+    return out
+
+
+def decode_append_into(q, k_cache, v_cache, k_new, v_new, n, scale, out, split=None, window=None, sink_tokens=0):
     """One decode step with the cache append fused in.
 
     k_cache/v_cache [B,Hkv,cap,D] (cap >= n), k_new/v_new [B,Hkv,1,D] or
     [B,Hkv,D]: the new rows are written to token n - 1 of the caches and q
-    attends over tokens [0, n). out [B,Hkv,G,D]. Enqueued on the current stream.
+    attends over tokens [0, n), with a ``window`` over the last `window` of them
+    and the first `sink_tokens`. out [B,Hkv,G,D]. Enqueued on the current stream.
     """
     _check_qkv(q, k_cache, v_cache, "decode_append")
     b, hkv, g, d = q.shape
@@ -161,26 +206,16 @@ def decode_append_into(q, k_cache, v_cache, k_new, v_new, n, scale, out, split=N
         raise ValueError(f"decode_append: n={n} outside [1, {k_cache.shape[2]}]")
     if out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise ValueError("decode_append: out must match q")
-    lib = _lib.load()
-    _, nbytes = _plan(q.device.index, b, hkv, g, d, int(n), split, False)
-    with _on_device(q.device):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        st2 = lambda t: _lib.i64x2(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
-        rc = lib.tc_decode_append_attention(
-            q.data_ptr(), _strides3(q), k_cache.data_ptr(), _strides3(k_cache, True), v_cache.data_ptr(),
-            _strides3(v_cache, True), kn.data_ptr(), st2(kn), vn.data_ptr(), st2(vn), int(n),
-            b, hkv, g, d, _lib.dtype_code(q.dtype), float(scale), int(split or 0),
-            ws.data_ptr(), ws.numel(), out.data_ptr(), _strides3(out), _lib.stream_of(q.device))
-        _lib.check(rc, "tc_decode_append_attention")
-    return out
+    return _append(q, k_cache, v_cache, kn, vn, None, int(n), scale, out, split, window, sink_tokens, "decode_append")
 
 
-def decode_append_at(q, k_cache, v_cache, k_new, v_new, pos, scale, out, split=None):
+def decode_append_at(q, k_cache, v_cache, k_new, v_new, pos, scale, out, split=None, window=None, sink_tokens=0):
     """decode_append_into with the append position on the device (graph-capturable).
 
     pos: int32 [B] on the device, the number of tokens already cached per
     sequence: the new rows go to token pos[b] of k_cache/v_cache [B,Hkv,cap,D]
-    and q attends over tokens [0, pos[b]]. Nothing here reads pos on the host,
+    and q attends over tokens [0, pos[b]] (or a ``window`` of them, as in
+    decode_append_into). Nothing here reads pos on the host,
     so a captured graph of this call stays valid while pos advances. The split
     plan depends on cap only.
     """
@@ -197,25 +232,14 @@ def decode_append_at(q, k_cache, v_cache, k_new, v_new, pos, scale, out, split=N
         raise ValueError("decode_append_at: pos must be a contiguous int32 [B] tensor on the device")
     if out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise ValueError("decode_append_at: out must match q")
-    cap = k_cache.shape[2]
-    lib = _lib.load()
-    _, nbytes = _plan(q.device.index, b, hkv, g, d, int(cap), split, False)
-    with _on_device(q.device):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        st2 = lambda t: _lib.i64x2(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
-        rc = lib.tc_decode_append_attention_at(
-            q.data_ptr(), _strides3(q), k_cache.data_ptr(), _strides3(k_cache, True), v_cache.data_ptr(),
-            _strides3(v_cache, True), kn.data_ptr(), st2(kn), vn.data_ptr(), st2(vn), pos.data_ptr(), int(cap),
-            b, hkv, g, d, _lib.dtype_code(q.dtype), float(scale), int(split or 0),
-            ws.data_ptr(), ws.numel(), out.data_ptr(), _strides3(out), _lib.stream_of(q.device))
-        _lib.check(rc, "tc_decode_append_attention_at")
-    return out
+    return _append(q, k_cache, v_cache, kn, vn, pos, int(k_cache.shape[2]), scale, out, split, window, sink_tokens,
+                   "decode_append_at")
 
 
-def decode_attention_batched(q, k, v, scale, lens=None, split=None):
-    """Batched form: q [B,Hkv,G,D], k/v [B,Hkv,N,D] → [B,Hkv,G,D] in q.dtype."""
+def decode_attention_batched(q, k, v, scale, lens=None, split=None, window=None, sink_tokens=0):
+    """Batched form: q [B,Hkv,G,D], k/v [B,Hkv,N,D] → [B,Hkv,G,D] in q.dtype; the rest as in decode_into."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    return decode_into(q, k, v, scale, out, lens=lens, split=split)
+    return decode_into(q, k, v, scale, out, lens=lens, split=split, window=window, sink_tokens=sink_tokens)
 
 
 def decode_attention(q, k, v, scale, split=None, block=16):

@@ -39,7 +39,7 @@ from transformers.cache_utils import DynamicLayer
 from . import _lib
 from .flash_decode import HEAD_DIM, _on_device, _plan
 from .kv import _plain, rope_table, rotate_half, rows_ok, watched
-from .prefill import GROUPS
+from .prefill import GROUPS, band_mask
 
 TILE = 16  # rows per tile-table entry (the decode kernel's tile)
 _I64P = ctypes.POINTER(ctypes.c_int64)
@@ -274,10 +274,19 @@ class PageTable:
         i = np.arange(len(rep)) - np.repeat(np.cumsum(fr[:, 2]) - fr[:, 2], fr[:, 2])
         return np.stack([fr[rep, 0], fr[rep, 1] + i], axis=1)
 
-    def tile_table(self):
+    def visible(self, b, window, sink_tokens):
+        """The fragments of sequence b's last `window` tokens and its first `sink_tokens`."""
+        n = self.length(b)
+        if n - window <= sink_tokens:
+            return self.frags[b]
+        return np.concatenate([_cut(self.frags[b], 0, sink_tokens), _cut(self.frags[b], n - window, n)])
+
+    def tile_table(self, window=None, sink_tokens=0):
         """int32 [B, max_tiles, 4] and tiles int32 [B] (numpy): entries {page, first slot,
-        rows, first logical position} in logical order."""
-        per = [_tiles(f, self.page_tokens) for f in self.frags]
+        rows, first logical position} in logical order. With a window, of the visible tokens
+        (positions then count those)."""
+        frags = self.frags if window is None else [self.visible(b, window, sink_tokens) for b in range(self.batch)]
+        per = [_tiles(f, self.page_tokens) for f in frags]
         mt = max(1, max(len(t) for t in per))
         tab = np.zeros((self.batch, mt, 4), dtype=np.int32)
         cnt = np.zeros(self.batch, dtype=np.int32)
@@ -326,7 +335,7 @@ class PagedKV:
         self.device = self.k_pools[0].device if self.k_pools else torch.device(
             "cuda", torch.cuda.current_device() if dev.index is None else dev.index)
         # (version, what device_table or device_offsets returns, for each stream)
-        self._dev_table = self._dev_off = (None, None)
+        self._dev_table = self._dev_off = self._dev_window = (None, None)
 
     @property
     def layers(self):
@@ -455,8 +464,27 @@ class PagedKV:
         return (copies.get(_lib.raw_stream(self.device.index))
                 or _lib.per_stream(copies, self.device.index, self._upload_table))
 
-    def _upload_table(self):
-        tab, cnt = self.table.tile_table()
+    def window_table(self, window, sink_tokens, what):
+        """device_table of the tokens that a sliding window shows each sequence's newest token: its last `window` and
+        its first `sink_tokens`. Attention over a set of keys does not depend on their order, so the decode kernels
+        take it like the whole table. One table serves every layer of a step."""
+        if window is None and not sink_tokens:
+            return self.device_table()
+        version, tables = self._dev_window
+        if version != self.table.version:
+            tables = {}
+            self._dev_window = (self.table.version, tables)
+        copies = tables.get((window, sink_tokens))
+        if copies is None:  # False: the window hides nothing
+            most = max(map(self.table.length, range(self.table.batch)))
+            copies = tables[window, sink_tokens] = {} if _lib.check_window(window, sink_tokens, most, what) else False
+        if copies is False:
+            return self.device_table()
+        return (copies.get(_lib.raw_stream(self.device.index))
+                or _lib.per_stream(copies, self.device.index, lambda: self._upload_table(window, sink_tokens)))
+
+    def _upload_table(self, window=None, sink_tokens=0):
+        tab, cnt = self.table.tile_table(window, sink_tokens)
         return _to_device(tab, self.device), _to_device(cnt, self.device), tab.shape[1]
 
     def device_offsets(self):
@@ -475,11 +503,12 @@ class PagedKV:
         off = self.table.token_offsets(st[0] * 2, st[2] * 2)
         return _to_device(off, self.device), off.shape[1]
 
-    def prefill(self, layer, query, scale, mask=None, causal=False, out=None):
+    def prefill(self, layer, query, scale, mask=None, causal=False, out=None, window=None, sink_tokens=0):
         """The prefill branch of threadcut/attention.py:43-46 over the pools: query
         [B, Hq, q, D] (any strides, last dim contiguous) attends the first n keys of every
         sequence (n = the sequences' common length; the last q of them are the queries'
-        own tokens), in logical order, with no mask, is_causal, or a boolean mask
+        own tokens), in logical order, with no mask, is_causal (and then, with a ``window``,
+        only the last `window` keys up to its own and the first `sink_tokens`), or a boolean mask
         [B|1, 1, q, n]. Returns [B, q, Hq, D] (the reference's transposed output)."""
         from . import prefill as pf
 
@@ -500,6 +529,9 @@ class PagedKV:
             return out
         if mask is not None and causal:
             raise ValueError("PagedKV.prefill: pass either a mask or causal")
+        if window is not None and not causal:
+            raise ValueError("PagedKV.prefill: a window needs causal (a mask holds its own)")
+        w = _lib.check_window(window, sink_tokens, n, "PagedKV.prefill")
         off, pitch = self.device_offsets()
         tiles, tiles_bytes, mptr, mst = None, 0, None, _lib.i64x3(0, 0, 1)
         if mask is not None:
@@ -516,9 +548,18 @@ class PagedKV:
         lib = _lib.load()
         kp, vp = self.k_pools[layer], self.v_pools[layer]
         with torch.cuda.device(self.device):
-            splits = pf.num_splits(b, ql, n, hq, self.kv_heads)
+            splits = (pf.num_splits(b, ql, n, hq, self.kv_heads) if w is None
+                      else pf.window_splits(b, ql, n, *w, hq, self.kv_heads))
             nbytes = lib.tc_prefill_workspace_bytes(b, ql, hq, splits)
             ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
+            if w is not None:
+                rc = lib.tc_prefill_paged_window_attention(
+                    query.data_ptr(), pf._strides(query, (0, 1, 2)), kp.data_ptr(), vp.data_ptr(), self._strides(),
+                    kp.shape[0], off.data_ptr(), pitch, *w, ql, n, b, hq, self.kv_heads, d,
+                    _lib.dtype_code(self.dtype), float(scale), splits, ws.data_ptr(), ws.numel(), out.data_ptr(),
+                    pf._strides(out, (0, 1, 2)), _lib.stream_of(self.device))
+                _lib.check(rc, "tc_prefill_paged_window_attention")
+                return out
             rc = lib.tc_prefill_paged_attention(
                 query.data_ptr(), pf._strides(query, (0, 1, 2)), kp.data_ptr(), vp.data_ptr(), self._strides(),
                 kp.shape[0], off.data_ptr(), pitch, mptr, mst,
@@ -553,8 +594,9 @@ class PagedKV:
             self.table.prune(b, n - self._step[2], n, 0)
         self._step = None
 
-    def decode(self, layer, q, scale, out=None, split=None):
-        """softmax(q·Kᵀ·scale)·V over each sequence's keys of one layer.
+    def decode(self, layer, q, scale, out=None, split=None, window=None, sink_tokens=0):
+        """softmax(q·Kᵀ·scale)·V over each sequence's keys of one layer, with a ``window``
+        over its last `window` ones and its first `sink_tokens`.
 
         q [B, Hkv, G, D] (G query heads per KV head, last dim contiguous) in the
         pools' dtype; returns out [B, Hkv, G, D]. Enqueued on the current stream.
@@ -574,7 +616,7 @@ class PagedKV:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
             raise ValueError("PagedKV.decode: out must match q in shape, dtype and device")
-        tab, cnt, mt = self.device_table()
+        tab, cnt, mt = self.window_table(window, sink_tokens, "decode")
         lib = _lib.load()
         kp, vp = self.k_pools[layer], self.v_pools[layer]
         _, nbytes = _plan(q.device.index, b, hkv, g, d, TILE * mt, split, b > 1)
@@ -652,18 +694,19 @@ class PagedKV:
         step[1].discard(layer)
         return out
 
-    def decode_append(self, layer, q, k_new, v_new, scale, out=None, split=None):
+    def decode_append(self, layer, q, k_new, v_new, scale, out=None, split=None, window=None, sink_tokens=0):
         """One decode step of one layer with the append fused in: k_new/v_new
         [B, Hkv, D] (or [B, Hkv, 1, D]) go to the slots `reserve_step` took, and q
-        attends every key of its sequence including the new one. Returns out
-        [B, Hkv, G, D]."""
+        attends every key of its sequence including the new one, or with a ``window`` the
+        last `window` of them, the new one among them, and the first `sink_tokens`. Returns
+        out [B, Hkv, G, D]."""
         step, fast = getattr(self, "_step", None), _lib.FAST
         if step is not None and step[2] != 1 and step[0] == self.table.version:
             raise RuntimeError(f"PagedKV.decode_append: the step has {step[2]} tokens a sequence (write_step takes them)")
         if (fast is not None and split is None and q.is_cuda and step is not None and step[0] == self.table.version
                 and layer in step[1]):
             # The whole call in native code; None for what it does not take (then as below).
-            tab, cnt, _ = self.device_table()
+            tab, cnt, _ = self.window_table(window, sink_tokens, "decode_append")
             done = fast.paged_append(q, self.k_pools[layer], self.v_pools[layer], tab, cnt, k_new, v_new, out, scale,
                                      _lib.raw_stream(q.get_device()))
             if done is not None:
@@ -690,7 +733,7 @@ class PagedKV:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
             raise ValueError("PagedKV.decode_append: out must match q in shape, dtype and device")
-        tab, cnt, mt = self.device_table()
+        tab, cnt, mt = self.window_table(window, sink_tokens, "decode_append")
         lib = _lib.load()
         kp, vp = self.k_pools[layer], self.v_pools[layer]
         _, nbytes = _plan(q.device.index, b, hkv, g, d, TILE * mt, split, b > 1)
@@ -934,8 +977,9 @@ def state_of(cache):
     return None
 
 
-def attention(layer, query, attention_mask, scaling):
-    """The "threadcut" attention for a paged layer: query [B, Hq, q, D] -> [B, q, Hq, D]."""
+def attention(layer, query, attention_mask, scaling, window=None, sink_tokens=0):
+    """The "threadcut" attention for a paged layer: query [B, Hq, q, D] -> [B, q, Hq, D]. A window is that of a call
+    without a mask."""
     b, hq, q, d = query.shape
     kv = layer.kv
     hkv = kv.kv_heads
@@ -947,20 +991,25 @@ def attention(layer, query, attention_mask, scaling):
             k_new, v_new = layer.pending
             layer.pending = None
             if layer.owner.device_lens is not None:
+                if _lib.check_window(window, sink_tokens, layer.n, "paged cache") is not None:
+                    raise RuntimeError("paged cache: the captured decode step has no sliding window")
                 kv.decode_append_at(layer.index, qg, k_new, v_new, layer.owner.device_lens, scaling, out=og)
             else:
-                kv.decode_append(layer.index, qg, k_new, v_new, scaling, out=og)
+                kv.decode_append(layer.index, qg, k_new, v_new, scaling, out=og, window=window, sink_tokens=sink_tokens)
         else:
-            kv.decode(layer.index, qg, scaling, out=og)
+            kv.decode(layer.index, qg, scaling, out=og, window=window, sink_tokens=sink_tokens)
         return out
     layer.flush()
-    is_causal = attention_mask is None and q > 1 and q == layer.n
+    is_causal = attention_mask is None and q > 1 and (q == layer.n or window is not None)
     m = attention_mask
     if g in GROUPS and (m is None or (m.dtype == torch.bool and m.dim() == 4 and m.shape[1] == 1)):
-        return kv.prefill(layer.index, query, scaling, m, is_causal)
+        return kv.prefill(layer.index, query, scaling, m, is_causal, window=window if is_causal else None,
+                          sink_tokens=sink_tokens if is_causal else 0)
     # Other masks and group sizes: the reference's route (repeat_kv + SDPA) on the gathered keys.
     ks, vs = zip(*[kv.gather(layer.index, i) for i in range(b)])
     k, v = torch.stack(ks), torch.stack(vs)
+    if window is not None:
+        m, is_causal = band_mask(q, k.shape[2], window, sink_tokens, k.device), False
     out = F.scaled_dot_product_attention(query, k.repeat_interleave(g, 1), v.repeat_interleave(g, 1),
                                          attn_mask=m, scale=scaling, is_causal=is_causal)
     return out.transpose(1, 2).contiguous()

@@ -58,14 +58,33 @@ def num_splits(batch, q_len, n_tokens, q_heads, kv_heads):
     return s
 
 
-def prefill_attention(query, key, value, attention_mask=None, scale=None, is_causal=False, out=None, splits=None):
+def band_mask(q, n, window, sink_tokens, device):
+    """bool [1, 1, q, n]: what q queries at the end of n keys see through a sliding window with sink tokens."""
+    p = torch.arange(n - q, n, device=device)[:, None]
+    j = torch.arange(n, device=device)[None]
+    return ((j <= p) & ((j > p - window) | (j < sink_tokens)))[None, None]
+
+
+def window_splits(batch, q_len, n_tokens, window, sink_tokens, q_heads, kv_heads):
+    """num_splits of a windowed call."""
+    s = _lib.load().tc_prefill_window_num_splits(int(batch), int(q_len), int(n_tokens), int(window), int(sink_tokens),
+                                                 int(q_heads), int(kv_heads))
+    if s < 0:
+        _lib.check(-s, "tc_prefill_window_num_splits")
+    return s
+
+
+def prefill_attention(query, key, value, attention_mask=None, scale=None, is_causal=False, out=None, splits=None,
+                      window=None, sink_tokens=0):
     """SDPA(query, repeat_kv(key, g), repeat_kv(value, g), attention_mask, scale,
     is_causal).transpose(1, 2) without expanding K/V.
 
     query [b, hq, q, d], key/value [b, hkv, n, d] (any strides, contiguous last
     dim), attention_mask None or bool [b|1, 1, q, n] (True = attend).
     ``is_causal`` needs no mask and aligns the queries to the end of the keys
-    (identical to SDPA's when q == n). Returns out [b, q, hq, d] (a new
+    (identical to SDPA's when q == n); with a ``window`` each query then sees the
+    last `window` keys up to its own and the first `sink_tokens`, and tiles that
+    no query sees are not read. Returns out [b, q, hq, d] (a new
     contiguous tensor unless `out` is given). Rows with no visible key are 0.
     ``splits`` fixes the number of key splits (default: ``num_splits``); more
     than one adds a workspace of fp32 partials and a combine pass.
@@ -85,6 +104,9 @@ def prefill_attention(query, key, value, attention_mask=None, scale=None, is_cau
             raise ValueError(f"prefill_attention: {name} must have a contiguous last dimension")
     if attention_mask is not None and is_causal:
         raise ValueError("prefill_attention: pass either attention_mask or is_causal")
+    if window is not None and not is_causal:
+        raise ValueError("prefill_attention: a window needs is_causal (a mask holds its own)")
+    w = _lib.check_window(window, sink_tokens, n, "prefill_attention")
     if out is None:
         out = torch.empty((b, q, hq, d), dtype=query.dtype, device=query.device)
     elif out.shape != (b, q, hq, d) or out.dtype != query.dtype or out.device != query.device or out.stride(3) != 1:
@@ -104,9 +126,17 @@ def prefill_attention(query, key, value, attention_mask=None, scale=None, is_cau
     lib = _lib.load()
     # The library plans splits for the current device (its CU count).
     with torch.cuda.device(query.device):
-        s = int(splits) if splits else num_splits(b, q, n, hq, hkv)
+        s = int(splits) if splits else num_splits(b, q, n, hq, hkv) if w is None else window_splits(b, q, n, *w, hq, hkv)
         ws_bytes = lib.tc_prefill_workspace_bytes(b, q, hq, s)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
+        if w is not None:
+            rc = lib.tc_prefill_window_attention(
+                query.data_ptr(), _strides(query, (0, 1, 2)), key.data_ptr(), _strides(key, (0, 1, 2), 2),
+                value.data_ptr(), _strides(value, (0, 1, 2), 2), *w, q, n, b, hq, hkv, d,
+                _lib.dtype_code(query.dtype), float(scale), s, None if ws is None else ws.data_ptr(), ws_bytes,
+                out.data_ptr(), _strides(out, (0, 1, 2)), _lib.stream_of(query.device))
+            _lib.check(rc, "tc_prefill_window_attention")
+            return out
         rc = lib.tc_prefill_attention(
             query.data_ptr(), _strides(query, (0, 1, 2)), key.data_ptr(), _strides(key, (0, 1, 2), 2),
             value.data_ptr(), _strides(value, (0, 1, 2), 2), mask_ptr, mask_strides,
