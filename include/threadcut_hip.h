@@ -319,6 +319,48 @@ int tc_decode_paged_append_attention_at(const void* q_dev, const int64_t q_strid
                                         int split_tokens, void* workspace_dev, size_t workspace_bytes,
                                         void* out_dev, const int64_t out_strides[3], void* stream);
 
+/* Decode of a batch whose sequences share a prefix: query b attends the
+ * prefix_tokens tokens of the prefix (one K and one V [kv_heads, prefix_tokens,
+ * head_dim], element strides (head, token)) and then its own tokens, as
+ * tc_decode_attention reads them (k, v, lens, n_tokens; n_tokens or a length
+ * may be 0). The prefix is read once for the whole batch. Workspace:
+ * tc_decode_workspace_bytes of tc_decode_shared_num_splits splits. No
+ * counterpart in the reference. */
+int tc_decode_shared_attention(const void* q_dev, const int64_t q_strides[3],
+                               const void* k_prefix_dev, const int64_t k_prefix_strides[2],
+                               const void* v_prefix_dev, const int64_t v_prefix_strides[2],
+                               int64_t prefix_tokens,
+                               const void* k_dev, const int64_t k_strides[3],
+                               const void* v_dev, const int64_t v_strides[3],
+                               const int32_t* lens_dev, int64_t n_tokens,
+                               int batch, int kv_heads, int group, int head_dim, int dtype,
+                               float scale, void* workspace_dev, size_t workspace_bytes,
+                               void* out_dev, const int64_t out_strides[3], void* stream);
+
+/* The same over page pools: shared_table_dev holds the prefix's shared_tiles
+ * tiles, tile_table_dev / tiles_dev / max_tiles each sequence's own, all in the
+ * format and with the bounds of tc_decode_paged_attention. k_new_dev set: the
+ * step writes the new token's rows as tc_decode_paged_append_attention does
+ * (into the last row of the sequence's last own tile); NULL: it writes none.
+ * Workspace: prefix_tokens = 16 * shared_tiles, max_tokens = 16 * max_tiles,
+ * ragged = batch > 1. */
+int tc_decode_paged_shared_attention(const void* q_dev, const int64_t q_strides[3],
+                                     void* k_pool_dev, void* v_pool_dev,
+                                     const int64_t pool_strides[3], int num_pages, int page_tokens,
+                                     const int32_t* shared_table_dev, int64_t shared_tiles,
+                                     const int32_t* tile_table_dev, const int32_t* tiles_dev,
+                                     int64_t max_tiles, const void* k_new_dev,
+                                     const int64_t k_new_strides[2], const void* v_new_dev,
+                                     const int64_t v_new_strides[2], int batch, int kv_heads,
+                                     int group, int head_dim, int dtype, float scale,
+                                     void* workspace_dev, size_t workspace_bytes,
+                                     void* out_dev, const int64_t out_strides[3], void* stream);
+
+/* Splits of a shared-prefix call (the prefix's and the sequences' own), or a
+ * negative TC_ERR_* code. ragged: per-sequence lengths. */
+int tc_decode_shared_num_splits(int batch, int kv_heads, int group, int64_t prefix_tokens,
+                                int64_t max_tokens, int ragged);
+
 /* ------------------------------------------------------------------------ */
 /* RoPE delta-shift and suffix splice                                        */
 /*                                                                           */

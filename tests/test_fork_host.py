@@ -116,3 +116,45 @@ def test_rotated_append_validation():
     assert rope(h=40000) == _lib.TC_ERR_UNSUPPORTED
     assert rope(rows=0, slots=None, host=None) == rope(layers=0, slots=None) == _lib.TC_OK
     assert _placed([[4, 1], [5, 0]], 7).tolist() == [[4, 1, 7, 0], [5, 0, 8, 0]]
+
+
+def test_shared_tiles():
+    t = PageTable(40, 16, batch=3)
+    t.reserve(0, 70)
+    t.fork(0, 1, 70)
+    t.fork(0, 2, 40)
+    t.reserve(2, 5)
+    assert t.shared_tiles(*t.tile_table()) == 2  # the third tile has 16 rows in two sequences, 8 in the third
+    t.release(2)
+    assert t.shared_tiles(*t.tile_table()) == 0
+    t.fork(1, 2, 70)
+    assert t.shared_tiles(*t.tile_table()) == 5
+    for b in range(3):
+        t.reserve(b, 1)
+    assert t.shared_tiles(*t.tile_table()) == 5
+    assert PageTable(4, 16).shared_tiles(*PageTable(4, 16).tile_table()) == 0
+
+
+def test_shared_entry_refusals():
+    lib = _lib.load()
+    st = _lib.i64x3(1 << 24, 1 << 20, 128)
+    s2 = _lib.i64x2(1 << 20, 128)
+
+    def shared(prefix=100, n=0, d=128, g=4, q=4096, kp=8192, ps=s2):
+        return lib.tc_decode_shared_attention(q, st, kp, ps, 12288, s2, prefix, 4096, st, 4096, st, None, n, 2, 8, g, d, 0,
+                                              0.088, 4096, 1 << 20, 16384, st, None)
+
+    assert shared(prefix=-1) == shared(n=-1) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert shared(d=64) == shared(g=9) == _lib.TC_ERR_UNSUPPORTED
+    assert lib.tc_decode_shared_num_splits(0, 8, 4, 100, 0, 0) == -_lib.TC_ERR_INVALID_ARGUMENT
+    assert lib.tc_decode_shared_num_splits(2, 8, 4, 1 << 40, 0, 0) == -_lib.TC_ERR_INVALID_ARGUMENT
+
+    def pages(pages=4, P=16, table=4096, tiles=3, own=4096, max_tiles=2, kn=None, vn=None):
+        return lib.tc_decode_paged_shared_attention(4096, st, 8192, 12288, st, pages, P, table, tiles, own, own, max_tiles,
+                                                    kn, s2, vn, s2, 2, 8, 4, 128, 0, 0.088, 4096, 1 << 20, 16384, st, None)
+
+    assert pages(pages=0) == pages(P=0) == pages(table=None) == pages(own=None) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert pages(tiles=-1) == pages(max_tiles=-1) == pages(max_tiles=1 << 28) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert pages(table=4104) == pages(own=4104) == _lib.TC_ERR_ALIGNMENT
+    assert pages(kn=4096) == pages(kn=4096, vn=4096, max_tiles=0) == _lib.TC_ERR_INVALID_ARGUMENT
+    assert pages(kn=4100, vn=4096) == _lib.TC_ERR_ALIGNMENT

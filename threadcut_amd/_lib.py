@@ -80,6 +80,11 @@ SIGNATURES = {
                                         _I, _P, _S, _P, _I64P, _P]),
     "tc_decode_append_window_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64, _I64,
                                                _I64, _I, _I, _I, _I, _I, _F, _I, _P, _S, _P, _I64P, _P]),
+    "tc_decode_shared_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _I64, _P, _I64P, _P, _I64P, _P, _I64, _I, _I,
+                                        _I, _I, _I, _F, _P, _S, _P, _I64P, _P]),
+    "tc_decode_paged_shared_attention": (_I, [_P, _I64P, _P, _P, _I64P, _I, _I, _P, _I64, _P, _P, _I64, _P, _I64P, _P,
+                                              _I64P, _I, _I, _I, _I, _I, _F, _P, _S, _P, _I64P, _P]),
+    "tc_decode_shared_num_splits": (_I, [_I, _I, _I, _I64, _I64, _I]),
     "tc_decode_window_tokens": (_I64, [_I64, _I64, _I64]),
     "tc_prefill_window_attention": (_I, [_P, _I64P, _P, _I64P, _P, _I64P, _I64, _I64, _I64, _I64, _I, _I, _I, _I, _I,
                                          _F, _I, _P, _S, _P, _I64P, _P]),

@@ -37,7 +37,8 @@
 #include <algorithm>
 #include <mutex>
 
-#include "tc_common.hpp"
+#include "decode_tile.hpp"
+#include "shared.hpp"
 
 namespace tc {
 namespace {
@@ -45,9 +46,6 @@ namespace {
 // Tuning knobs (measured on MI355X; override with -D for sweeps).
 #ifndef TC_DECODE_WAVES
 #define TC_DECODE_WAVES 4   // waves per partial work-group
-#endif
-#ifndef TC_DECODE_AUX
-#define TC_DECODE_AUX 2     // cache-policy bits of the K/V buffer loads (2: non-temporal stream)
 #endif
 #ifndef TC_DECODE_INTERLEAVE
 #define TC_DECODE_INTERLEAVE 1  // tc_decode_attention deals tiles round-robin over the splits
@@ -68,7 +66,6 @@ namespace {
 #define TC_DECODE_STAMPS 0  // 1: the measurement build; every partial wave records a timeline
 #endif
 
-constexpr int kHeadDim = 128;
 constexpr int64_t kMaxTokens = int64_t(1) << 29;  // token positions stay 32-bit in the kernel
 constexpr int kWaves = TC_DECODE_WAVES;
 // Short caches (at most TC_DECODE_SHORT_TOKENS tokens, one length for the
@@ -78,24 +75,22 @@ constexpr int kWaves = TC_DECODE_WAVES;
 // 5.87, 1024 5.89 against 6.02, 1536 6.05 against 6.25, 2048 6.50 against
 // 6.84; at 3072 and 4096 tokens two waves are slower).
 constexpr int kShortWaves = 2;
-constexpr int kWaveIter = 16;                        // tokens per wave iteration
 constexpr int kSplitGranule = kWaves * kWaveIter > 64 ? kWaves * kWaveIter : 64;  // split length granule
 static_assert(kSplitGranule % (kShortWaves * kWaveIter) == 0, "short plans split at the same granule");
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 struct PartialArgs {
   const uint16_t* q;
   const uint16_t* k;
   const uint16_t* v;
-  float* o_part;       // [B, H, S, G, D]
-  float* lse_part;     // [B, H, S, G]
+  float* o_part;       // [B, H, part_splits, G, D]: this call's splits from part0 on
+  float* lse_part;     // [B, H, part_splits, G]
   const int32_t* lens; // [B] or null
   int64_t n;
   int64_t sq_b, sq_h, sq_g;
   int64_t sk_b, sk_h, sk_t;
   int64_t sv_b, sv_h, sv_t;
   int heads, group, splits, split_tokens;
+  int part_splits, part0;
   int interleave;      // 0: split s owns tokens [s*T, (s+1)*T); 1: 16-token tiles dealt round-robin
   int longest_first;   // per-sequence lengths, batch <= 64: work-group row z serves the z-th longest sequence
   float scale_log2;    // softmax scale * log2(e)
@@ -147,139 +142,6 @@ struct CombineArgs {
   int64_t so_b, so_h, so_g;
   int heads, group, splits;
 };
-
-// Reductions over the four 16-lane rows of a wave (every lane gets the result).
-// v_permlane16_swap(x, x) leaves rows (x0, x0, x2, x2) and (x1, x1, x3, x3) in its two
-// results, so their sum is x0 + x1 (x2 + x3) in every lane; permlane32 pairs the halves.
-__device__ __forceinline__ float pair16_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float pair32_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float pair16_max(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float pair32_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float rows_sum(float x) { return pair32_sum(pair16_sum(x)); }
-__device__ __forceinline__ float rows_max(float x) { return pair32_max(pair16_max(x)); }
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
-// A wave-uniform read of memory that no kernel writes while this one runs:
-// through the constant address space it becomes a scalar load.
-__device__ __forceinline__ int32_t const_load(const int32_t* p) {
-  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
-}
-
-// Buffer resource over `bytes` bytes at p; loads past the end return zero.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, int32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
-}
-
-__device__ __forceinline__ uint4 bload16(__amdgpu_buffer_rsrc_t r, int32_t off) {
-  const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, TC_DECODE_AUX);
-  return make_uint4(v.x, v.y, v.z, v.w);
-}
-
-// K/V of one 16-token tile of a wave (lane l = 16 g + n): k[i] = token n,
-// dims 32 i + 8 g .. +8 (the A operand of QK block i); v[j] = token 4 g + j,
-// dims 8 n .. +8. Rows at or past `end` read as zero (their scores are
-// masked), so no index clamping is needed.
-struct Tile {
-  uint4 k[4];
-  uint4 v[4];
-  int32_t rows;  // paged cache: the tile's key rows (the rest read as zero)
-};
-
-__device__ __forceinline__ void load_tile(Tile& t, const char* kslab, const char* vslab, int32_t row_k,
-                                          int32_t row_v, int32_t t0, int32_t end, const int32_t* koff,
-                                          const int32_t* voff) {
-  // The clamp is wave-uniform, but i32 min/max select v_med3 (a VGPR);
-  // readfirstlane keeps the buffer resource in SGPRs (no waterfall loop).
-  const int32_t rows = __builtin_amdgcn_readfirstlane(min(max(end - t0, 0), 16));
-  const __amdgpu_buffer_rsrc_t rk = make_rsrc(kslab + static_cast<int64_t>(t0) * row_k, rows * row_k);
-  const __amdgpu_buffer_rsrc_t rv = make_rsrc(vslab + static_cast<int64_t>(t0) * row_v, rows * row_v);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    t.k[j] = bload16(rk, koff[j]);
-    t.v[j] = bload16(rv, voff[j]);
-  }
-}
-
-// Paged cache: rows (<= 16) key rows from slot `slot` of page `page`. The
-// buffer range spans exactly those rows, so the rest of the tile reads as
-// zero; an entry outside the pool or past the page's end loads nothing.
-__device__ __forceinline__ void load_paged_tile(Tile& t, const char* kpool, const char* vpool, int32_t row_k,
-                                                int32_t row_v, int64_t page_k, int64_t page_v, int32_t pages,
-                                                int32_t page_tokens, int32_t page, int32_t slot, int32_t rows,
-                                                const int32_t* koff, const int32_t* voff) {
-  if (page < 0 || page >= pages || slot < 0 || rows < 0 || rows > 16 || slot > page_tokens - rows) {
-    page = 0; slot = 0; rows = 0;
-  }
-  t.rows = rows;
-  const __amdgpu_buffer_rsrc_t rk = make_rsrc(kpool + page * page_k + static_cast<int64_t>(slot) * row_k, rows * row_k);
-  const __amdgpu_buffer_rsrc_t rv = make_rsrc(vpool + page * page_v + static_cast<int64_t>(slot) * row_v, rows * row_v);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    t.k[j] = bload16(rk, koff[j]);
-    t.v[j] = bload16(rv, voff[j]);
-  }
-}
-
-typedef _Float16 mfma_h4 __attribute__((ext_vector_type(4)));
-typedef _Float16 mfma_h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 mfma_b8 __attribute__((ext_vector_type(8)));
-typedef short mfma_s4 __attribute__((ext_vector_type(4)));
-typedef float mfma_f4 __attribute__((ext_vector_type(4)));
-
-template <int DT> struct DecodeMma;
-template <> struct DecodeMma<TC_DTYPE_F16> {
-  static __device__ __forceinline__ mfma_f4 qk(const uint4& a, const uint4& b, const mfma_f4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(mfma_h8, a), __builtin_bit_cast(mfma_h8, b), c,
-                                                  0, 0, 0);
-  }
-  static __device__ __forceinline__ mfma_f4 pv(const uint2& a, const uint2& b, const mfma_f4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(mfma_h4, a), __builtin_bit_cast(mfma_h4, b), c,
-                                                 0, 0, 0);
-  }
-  // Two fp32 values rounded to nearest even into one word (first in the low half).
-  static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const h2 v = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
-    return __builtin_bit_cast(uint32_t, v);
-  }
-};
-template <> struct DecodeMma<TC_DTYPE_BF16> {
-  static __device__ __forceinline__ mfma_f4 qk(const uint4& a, const uint4& b, const mfma_f4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mfma_b8, a), __builtin_bit_cast(mfma_b8, b), c,
-                                                   0, 0, 0);
-  }
-  static __device__ __forceinline__ mfma_f4 pv(const uint2& a, const uint2& b, const mfma_f4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(mfma_s4, a), __builtin_bit_cast(mfma_s4, b),
-                                                     c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const b2 v = {static_cast<__bf16>(x), static_cast<__bf16>(y)};
-    return __builtin_bit_cast(uint32_t, v);
-  }
-};
-
-// Row-major V tile in a wave's LDS region: 16 token rows of 256 bytes, each
-// padded to 288 so that the transposing reads (4 rows x 32 bytes per 16-lane
-// group, 16 rows per instruction) and the 16-byte row stores fall on distinct
-// banks.
-constexpr int kVRowBytes = 2 * kHeadDim + 32;
-constexpr int kVTileWords = 16 * kVRowBytes / 4;
-typedef short lds_s4 __attribute__((ext_vector_type(4)));
-constexpr float kLazyMax = 8.f;               // log2 units the running maximum may lag
 
 // APPEND: the kernel attends (and writes) the new token of an append call
 // (a.k_new != null); DIRECT: it writes the result (a.out != null), of one
@@ -591,7 +453,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? 
 #endif
   // The head's sum over the four lane groups; m is already common to them.
   l = rows_sum(l);
-  const int64_t part = (static_cast<int64_t>(b) * a.heads + h) * a.splits + split;
+  const int64_t part = (static_cast<int64_t>(b) * a.heads + h) * a.part_splits + a.part0 + split;
   static_assert(W > 1, "the waves of a work-group are merged below");
   if (n < a.group) {
 #pragma unroll
@@ -980,7 +842,7 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
                  int kv_heads, int group, int head_dim, int dtype, float scale, int split_tokens, int num_splits,
                  float* o_part_dev, float* lse_part_dev, int interleave, const Append* app, void* stream,
                  const Paged* paged = nullptr, bool whole_call = false, void* out_dev = nullptr,
-                 const int64_t* out_strides = nullptr, const Window* window = nullptr) {
+                 const int64_t* out_strides = nullptr, const Window* window = nullptr, int part0 = 0) {
   int rc = check_common(batch, kv_heads, group, head_dim, dtype);
   if (rc != TC_OK) return rc;
   if (n_tokens == 0 && num_splits == 0) return TC_OK;  // empty caches: nothing to read
@@ -1029,6 +891,8 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
   a.group = group;
   a.splits = num_splits;
   a.split_tokens = split_tokens;
+  a.part0 = part0;
+  a.part_splits = part0 + num_splits;
   a.interleave = interleave;
   // Longest sequences first: only for per-sequence lengths of a contiguous
   // cache, and up to 64 sequences (one lane each).
@@ -1432,6 +1296,166 @@ int tc_decode_paged_append_attention_at(const void* q_dev, const int64_t q_strid
   return attention_impl(q_dev, q_strides, k_pool_dev, pool_strides, v_pool_dev, pool_strides, lens_dev,
                         16 * max_tiles, batch, kv_heads, group, head_dim, dtype, scale, split_tokens, workspace_dev,
                         workspace_bytes, out_dev, out_strides, &app, batch > 1, stream, &p);
+}
+
+}  // extern "C"
+
+namespace tc {
+namespace {
+
+// The prefix of a shared-prefix call: contiguous [H, tokens, D] of K and V with (head, token) strides, or tiles of the
+// page pools that hold every sequence's own tokens too.
+struct Prefix {
+  const void* k;
+  const int64_t* k_strides;
+  const void* v;
+  const int64_t* v_strides;
+  int64_t tokens;
+  const int32_t* tiles = nullptr;
+};
+
+// Splits of a shared-prefix call: the prefix pass's come first.
+int shared_plan(int batch, int kv_heads, int group, int64_t prefix_tokens, int64_t max_tokens, int ragged, int* S_prefix,
+                int* S_own, int* T_own) {
+  int cus = 0, rc;
+  if (batch < 1 || kv_heads < 1 || group < 1 || prefix_tokens < 0 || prefix_tokens > kMaxTokens)
+    return fail(TC_ERR_INVALID_ARGUMENT, "prefix of %lld tokens, batch %d, kv_heads %d, group %d",
+                (long long)prefix_tokens, batch, kv_heads, group);
+  if ((rc = split_plan(batch, kv_heads, max_tokens, 0, ragged, S_own, T_own)) != TC_OK) return rc;
+  *S_prefix = 0;
+  if (prefix_tokens == 0) return TC_OK;
+  if ((rc = current_device_cus(&cus)) != TC_OK) return rc;
+  *S_prefix = prefix_splits(batch, kv_heads, group, ceil_div(prefix_tokens, kWaveIter), cus);
+  return TC_OK;
+}
+
+int shared_impl(const void* q_dev, const int64_t q_strides[3], const Prefix& x, const void* k_dev,
+                const int64_t k_strides[3], const void* v_dev, const int64_t v_strides[3], const int32_t* lens_dev,
+                int64_t n_tokens, int batch, int kv_heads, int group, int head_dim, int dtype, float scale,
+                void* workspace_dev, size_t workspace_bytes, void* out_dev, const int64_t out_strides[3],
+                const Append* app, int ragged, void* stream, const Paged* paged) {
+  int rc = check_common(batch, kv_heads, group, head_dim, dtype);
+  if (rc != TC_OK) return rc;
+  if (n_tokens < 0) return fail(TC_ERR_INVALID_ARGUMENT, "n_tokens %lld is negative", (long long)n_tokens);
+  if (x.tokens == 0)
+    return attention_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch, kv_heads,
+                          group, head_dim, dtype, scale, 0, workspace_dev, workspace_bytes, out_dev, out_strides, app,
+                          ragged, stream, paged);
+  int Sp = 0, S = 0, t = 0;
+  if ((rc = shared_plan(batch, kv_heads, group, x.tokens, n_tokens, ragged, &Sp, &S, &t)) != TC_OK) return rc;
+  if (!q_dev || !x.k || !x.v || !out_dev) return fail(TC_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned16(q_dev) || !aligned16(x.k) || !aligned16(x.v) || !aligned16(out_dev) || !aligned16(workspace_dev))
+    return fail(TC_ERR_ALIGNMENT, "q/k/v/out/workspace base pointers must be 16-byte aligned");
+  if ((rc = check_strides("q", q_strides, 3)) != TC_OK) return rc;
+  if ((rc = check_strides("out", out_strides, 3)) != TC_OK) return rc;
+  if ((rc = check_strides("prefix k", x.k_strides, x.tiles ? 3 : 2)) != TC_OK) return rc;
+  if ((rc = check_strides("prefix v", x.v_strides, x.tiles ? 3 : 2)) != TC_OK) return rc;
+  const int64_t sk_t = x.k_strides[x.tiles ? 2 : 1], sv_t = x.v_strides[x.tiles ? 2 : 1];
+  constexpr int64_t kMaxTokenStride = int64_t(1) << 26;  // a tile's 16 rows in 32-bit offsets
+  if (sk_t < head_dim || sv_t < head_dim || sk_t >= kMaxTokenStride || sv_t >= kMaxTokenStride)
+    return fail(TC_ERR_INVALID_ARGUMENT, "prefix token strides (%lld, %lld) outside [%d, 2^26)", (long long)sk_t,
+                (long long)sv_t, head_dim);
+  if (!isfinite(scale)) return fail(TC_ERR_INVALID_ARGUMENT, "scale is not finite");
+  const size_t need = tc_decode_workspace_bytes(batch, kv_heads, group, head_dim, Sp + S);
+  if (!workspace_dev || workspace_bytes < need)
+    return fail(TC_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed for %d splits", workspace_bytes, need, Sp + S);
+  float* o_part = static_cast<float*>(workspace_dev);
+  float* lse_part = o_part + static_cast<size_t>(batch) * kv_heads * (Sp + S) * group * head_dim;
+  // The own tokens first: their arguments are checked there, and nothing is enqueued if they are refused.
+  if (S > 0 && (rc = partial_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch,
+                                  kv_heads, group, head_dim, dtype, scale, t, S, o_part, lse_part, 1, app, stream,
+                                  paged, true, nullptr, nullptr, nullptr, Sp)) != TC_OK) return rc;
+  PrefixArgs a;
+  a.q = static_cast<const uint16_t*>(q_dev);
+  a.k = static_cast<const uint16_t*>(x.k);
+  a.v = static_cast<const uint16_t*>(x.v);
+  a.o_part = o_part;
+  a.lse_part = lse_part;
+  a.sq_b = q_strides[0]; a.sq_h = q_strides[1]; a.sq_g = q_strides[2];
+  a.sk_p = x.tiles ? x.k_strides[0] : 0;
+  a.sv_p = x.tiles ? x.v_strides[0] : 0;
+  a.sk_h = x.k_strides[x.tiles ? 1 : 0];
+  a.sv_h = x.v_strides[x.tiles ? 1 : 0];
+  a.sk_t = sk_t;
+  a.sv_t = sv_t;
+  a.tile_tab = x.tiles;
+  a.tiles = static_cast<int32_t>(ceil_div(x.tokens, kWaveIter));
+  a.n = static_cast<int32_t>(x.tokens);
+  a.pages = paged ? paged->pages : 0;
+  a.page_tokens = paged ? paged->page_tokens : 0;
+  a.heads = kv_heads;
+  a.group = group;
+  a.batch = batch;
+  a.splits = Sp;
+  a.part_splits = Sp + S;
+  a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  if ((rc = hip_status(launch_prefix(a, dtype, static_cast<hipStream_t>(stream)), "prefix pass launch")) != TC_OK) return rc;
+  return tc_decode_combine(o_part, lse_part, batch, kv_heads, group, head_dim, Sp + S, out_dev, out_strides, dtype,
+                           stream);
+}
+
+}  // namespace
+}  // namespace tc
+
+extern "C" {
+
+int tc_decode_shared_num_splits(int batch, int kv_heads, int group, int64_t prefix_tokens, int64_t max_tokens,
+                                int ragged) {
+  clear_error();
+  int Sp = 0, S = 0, t = 0;
+  const int rc = shared_plan(batch, kv_heads, group, prefix_tokens, max_tokens, ragged, &Sp, &S, &t);
+  return rc == TC_OK ? Sp + S : -rc;
+}
+
+int tc_decode_shared_attention(const void* q_dev, const int64_t q_strides[3], const void* k_prefix_dev,
+                               const int64_t k_prefix_strides[2], const void* v_prefix_dev,
+                               const int64_t v_prefix_strides[2], int64_t prefix_tokens, const void* k_dev,
+                               const int64_t k_strides[3], const void* v_dev, const int64_t v_strides[3],
+                               const int32_t* lens_dev, int64_t n_tokens, int batch, int kv_heads, int group,
+                               int head_dim, int dtype, float scale, void* workspace_dev, size_t workspace_bytes,
+                               void* out_dev, const int64_t out_strides[3], void* stream) {
+  clear_error();
+  const Prefix x{k_prefix_dev, k_prefix_strides, v_prefix_dev, v_prefix_strides, prefix_tokens};
+  return shared_impl(q_dev, q_strides, x, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch, kv_heads,
+                     group, head_dim, dtype, scale, workspace_dev, workspace_bytes, out_dev, out_strides, nullptr,
+                     lens_dev != nullptr, stream, nullptr);
+}
+
+int tc_decode_paged_shared_attention(const void* q_dev, const int64_t q_strides[3], void* k_pool_dev, void* v_pool_dev,
+                                     const int64_t pool_strides[3], int num_pages, int page_tokens,
+                                     const int32_t* shared_table_dev, int64_t shared_tiles,
+                                     const int32_t* tile_table_dev, const int32_t* tiles_dev, int64_t max_tiles,
+                                     const void* k_new_dev, const int64_t k_new_strides[2], const void* v_new_dev,
+                                     const int64_t v_new_strides[2], int batch, int kv_heads, int group, int head_dim,
+                                     int dtype, float scale, void* workspace_dev, size_t workspace_bytes,
+                                     void* out_dev, const int64_t out_strides[3], void* stream) {
+  clear_error();
+  if (num_pages < 1 || page_tokens < 1)
+    return fail(TC_ERR_INVALID_ARGUMENT, "pool of %d pages of %d tokens", num_pages, page_tokens);
+  if (max_tiles < 0 || max_tiles > kMaxTokens / 16 || shared_tiles < 0 || shared_tiles > kMaxTokens / 16)
+    return fail(TC_ERR_INVALID_ARGUMENT, "tables of %lld and %lld tiles", (long long)shared_tiles, (long long)max_tiles);
+  if ((max_tiles > 0 && (!tile_table_dev || !tiles_dev)) || (shared_tiles > 0 && !shared_table_dev))
+    return fail(TC_ERR_INVALID_ARGUMENT, "null tile table");
+  if (!aligned16(tile_table_dev) || !aligned16(shared_table_dev))
+    return fail(TC_ERR_ALIGNMENT, "tile table not 16-byte aligned");
+  if (!pool_strides) return fail(TC_ERR_INVALID_ARGUMENT, "null pool strides");
+  const Append app{k_new_dev, k_new_strides, v_new_dev, v_new_strides, k_pool_dev, v_pool_dev};
+  if (k_new_dev || v_new_dev) {
+    if (max_tiles < 1) return fail(TC_ERR_INVALID_ARGUMENT, "append without tiles of the sequences' own");
+    if (!k_new_dev || !v_new_dev || !k_new_strides || !v_new_strides)
+      return fail(TC_ERR_INVALID_ARGUMENT, "null new-token K/V");
+    if (!aligned16(k_new_dev) || !aligned16(v_new_dev))
+      return fail(TC_ERR_ALIGNMENT, "new-token K/V not 16-byte aligned");
+    for (int i = 0; i < 2; ++i)
+      if (k_new_strides[i] < 0 || v_new_strides[i] < 0 || k_new_strides[i] % 8 || v_new_strides[i] % 8)
+        return fail(TC_ERR_ALIGNMENT, "new-token K/V strides must be non-negative multiples of 8");
+  }
+  const Paged p{tile_table_dev, tiles_dev, max_tiles, num_pages, page_tokens};
+  const Prefix x{k_pool_dev, pool_strides, v_pool_dev, pool_strides, 16 * shared_tiles,
+                 shared_tiles ? shared_table_dev : nullptr};
+  return shared_impl(q_dev, q_strides, x, k_pool_dev, pool_strides, v_pool_dev, pool_strides, nullptr, 16 * max_tiles,
+                     batch, kv_heads, group, head_dim, dtype, scale, workspace_dev, workspace_bytes, out_dev,
+                     out_strides, k_new_dev ? &app : nullptr, batch > 1, stream, &p);
 }
 
 }  // extern "C"

@@ -242,6 +242,58 @@ def decode_attention_batched(q, k, v, scale, lens=None, split=None, window=None,
     return decode_into(q, k, v, scale, out, lens=lens, split=split, window=window, sink_tokens=sink_tokens)
 
 
+@functools.lru_cache(maxsize=1024)
+def _shared_workspace(device_index, b, hkv, g, d, prefix, n, ragged):
+    """Workspace bytes of a shared-prefix call, planned for the device as _plan does."""
+    lib = _lib.load()
+    with torch.cuda.device(device_index):
+        s = lib.tc_decode_shared_num_splits(b, hkv, g, prefix, n, int(bool(ragged)))
+    if s < 0:
+        _lib.check(-s, "tc_decode_shared_num_splits")
+    return max(lib.tc_decode_workspace_bytes(b, hkv, g, d, s), 16)
+
+
+def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lens=None, out=None):
+    """Decode of a batch whose sequences share a prefix: out[b,h,g] = softmax(q·[Kp; K_b]ᵀ·scale)·[Vp; V_b].
+
+    q [B,Hkv,G,D]; k_prefix/v_prefix [Hkv,P,D] or [1,Hkv,P,D], the tokens that
+    every sequence begins with; k/v [B,Hkv,N,D] each sequence's own tokens
+    behind them (N may be 0), of which lens (int32 [B] on the device, each
+    0..N) count, or all. The prefix is read once for the whole batch. Returns
+    out [B,Hkv,G,D] (a new tensor unless given). Enqueued on the current stream.
+    """
+    _check_qkv(q, k, v, "decode_attention_shared")
+    _lib.require_gpu(k_prefix, v_prefix, what="decode_attention_shared")
+    b, hkv, g, d = q.shape
+    kp, vp = (t[0] if t.dim() == 4 and t.shape[0] == 1 else t for t in (k_prefix, v_prefix))
+    if kp.dim() != 3 or kp.shape != vp.shape or kp.shape[0] != hkv or kp.shape[2] != d:
+        raise ValueError(f"decode_attention_shared: prefix {tuple(k_prefix.shape)}, {tuple(v_prefix.shape)} does not fit "
+                         f"q {tuple(q.shape)}")
+    for t in (kp, vp):
+        if t.dtype != q.dtype or t.device != q.device or t.stride(2) != 1:
+            raise ValueError("decode_attention_shared: the prefix must be in q's dtype and device, last dim contiguous")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
+        raise ValueError("decode_attention_shared: out must match q in shape, dtype and device")
+    if lens is not None and (lens.dtype != torch.int32 or lens.device != q.device or lens.shape != (b,)
+                             or not lens.is_contiguous()):
+        raise ValueError("decode_attention_shared: lens must be a contiguous int32 [B] tensor on the device")
+    n, prefix = k.shape[2], kp.shape[1]
+    lib = _lib.load()
+    st2 = lambda t: _lib.i64x2(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else d)
+    nbytes = _shared_workspace(q.device.index, b, hkv, g, d, prefix, n, lens is not None)
+    with _on_device(q.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        rc = lib.tc_decode_shared_attention(
+            q.data_ptr(), _strides3(q), kp.data_ptr(), st2(kp), vp.data_ptr(), st2(vp), prefix, k.data_ptr(),
+            _strides3(k, True), v.data_ptr(), _strides3(v, True), lens.data_ptr() if lens is not None else None, n,
+            b, hkv, g, d, _lib.dtype_code(q.dtype), float(scale), ws.data_ptr(), ws.numel(), out.data_ptr(),
+            _strides3(out), _lib.stream_of(q.device))
+        _lib.check(rc, "tc_decode_shared_attention")
+    return out
+
+
 def decode_attention(q, k, v, scale, split=None, block=16):
     """q: [hkv, g, d]; k, v: [hkv, n, d] (last dim contiguous). Returns [hkv, g, d].
 

@@ -37,11 +37,12 @@ from transformers import DynamicCache
 from transformers.cache_utils import DynamicLayer
 
 from . import _lib
-from .flash_decode import HEAD_DIM, _on_device, _plan
+from .flash_decode import HEAD_DIM, _on_device, _plan, _shared_workspace
 from .kv import _plain, rope_table, rotate_half, rows_ok, watched
 from .prefill import GROUPS, band_mask
 
 TILE = 16  # rows per tile-table entry (the decode kernel's tile)
+SHARED_MIN_TOKENS = 256  # tokens that all sequences share, from which decode reads them once for all
 _I64P = ctypes.POINTER(ctypes.c_int64)
 
 
@@ -295,6 +296,12 @@ class PageTable:
             cnt[b] = len(ts)
         return tab, cnt
 
+    def shared_tiles(self, tab, cnt):
+        """Leading tiles of a tile_table that are the same in every sequence."""
+        most = int(cnt.min()) if self.users and self.batch > 1 else 0
+        apart = (tab[:, :most, :3] != tab[:1, :most, :3]).any(axis=(0, 2))
+        return int(apart.argmax()) if apart.any() else most
+
     def token_offsets(self, page_bytes, slot_bytes, pitch=None):
         """int32 [B, pitch]: byte offset of every logical token's row within a head slab of
         the pools (page * page_bytes + slot * slot_bytes); past a sequence's end, INT32_MIN,
@@ -335,7 +342,7 @@ class PagedKV:
         self.device = self.k_pools[0].device if self.k_pools else torch.device(
             "cuda", torch.cuda.current_device() if dev.index is None else dev.index)
         # (version, what device_table or device_offsets returns, for each stream)
-        self._dev_table = self._dev_off = self._dev_window = (None, None)
+        self._dev_table = self._dev_off = self._dev_window = self._dev_shared = (None, None)
 
     @property
     def layers(self):
@@ -463,6 +470,41 @@ class PagedKV:
             self._dev_table = (self.table.version, copies)
         return (copies.get(_lib.raw_stream(self.device.index))
                 or _lib.per_stream(copies, self.device.index, self._upload_table))
+
+    def shared_tables(self):
+        """(the tiles that every sequence begins with, int32 [T, 4], each sequence's own in device_table's form, on
+        the device) of a cache with forked sequences, or None where they share less than pays."""
+        if not self.table.users:
+            return None
+        version, copies = self._dev_shared
+        if version != self.table.version:
+            tab, cnt = self.table.tile_table()
+            t = self.table.shared_tiles(tab, cnt)
+            copies = (tab[0, :t], tab[:, t:], cnt - t, {}) if t * TILE >= SHARED_MIN_TOKENS else False
+            self._dev_shared = (self.table.version, copies)
+        if copies is False:
+            return None
+        head, own, cnt, streams = copies
+        return (streams.get(_lib.raw_stream(self.device.index)) or _lib.per_stream(
+            streams, self.device.index, lambda: tuple(_to_device(x, self.device) for x in (head, own, cnt))))
+
+    def _attend_shared(self, tables, layer, q, k_new, v_new, scale, out):
+        """decode (k_new None) or decode_append of checked tensors over shared_tables."""
+        head, own, cnt = tables
+        b, hkv, g, d = q.shape
+        kp, vp = self.k_pools[layer], self.v_pools[layer]
+        nbytes = _shared_workspace(self.device.index, b, hkv, g, d, TILE * head.shape[0], TILE * own.shape[1], b > 1)
+        st = lambda t: None if t is None else _lib.i64x2(t.stride(0), t.stride(1))
+        ptr = lambda t: None if t is None else t.data_ptr()
+        with _on_device(self.device):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            rc = _lib.load().tc_decode_paged_shared_attention(
+                q.data_ptr(), _lib.i64x3(*q.stride()[:3]), kp.data_ptr(), vp.data_ptr(), self._strides(), kp.shape[0],
+                kp.shape[2], head.data_ptr(), head.shape[0], own.data_ptr(), cnt.data_ptr(), own.shape[1],
+                ptr(k_new), st(k_new), ptr(v_new), st(v_new), b, hkv, g, d, _lib.dtype_code(self.dtype), float(scale),
+                ws.data_ptr(), ws.numel(), out.data_ptr(), _lib.i64x3(*out.stride()[:3]), _lib.stream_of(self.device))
+            _lib.check(rc, "tc_decode_paged_shared_attention")
+        return out
 
     def window_table(self, window, sink_tokens, what):
         """device_table of the tokens that a sliding window shows each sequence's newest token: its last `window` and
@@ -616,6 +658,9 @@ class PagedKV:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
             raise ValueError("PagedKV.decode: out must match q in shape, dtype and device")
+        tables = self.shared_tables() if window is None and split is None else None
+        if tables is not None:
+            return self._attend_shared(tables, layer, q, None, None, scale, out)
         tab, cnt, mt = self.window_table(window, sink_tokens, "decode")
         lib = _lib.load()
         kp, vp = self.k_pools[layer], self.v_pools[layer]
@@ -704,7 +749,7 @@ class PagedKV:
         if step is not None and step[2] != 1 and step[0] == self.table.version:
             raise RuntimeError(f"PagedKV.decode_append: the step has {step[2]} tokens a sequence (write_step takes them)")
         if (fast is not None and split is None and q.is_cuda and step is not None and step[0] == self.table.version
-                and layer in step[1]):
+                and layer in step[1] and not self.table.users):
             # The whole call in native code; None for what it does not take (then as below).
             tab, cnt, _ = self.window_table(window, sink_tokens, "decode_append")
             done = fast.paged_append(q, self.k_pools[layer], self.v_pools[layer], tab, cnt, k_new, v_new, out, scale,
@@ -733,6 +778,11 @@ class PagedKV:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
             raise ValueError("PagedKV.decode_append: out must match q in shape, dtype and device")
+        tables = self.shared_tables() if window is None and split is None else None
+        if tables is not None:
+            self._attend_shared(tables, layer, q, kn, vn, scale, out)
+            step[1].discard(layer)
+            return out
         tab, cnt, mt = self.window_table(window, sink_tokens, "decode_append")
         lib = _lib.load()
         kp, vp = self.k_pools[layer], self.v_pools[layer]
