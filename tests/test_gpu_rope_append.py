@@ -1,6 +1,8 @@
 """Rotated appends into a paged cache (tc_paged_append_rope): the keys and queries of new tokens are rotated to their
 positions on the way, against the rotation in float64; values are copied bit for bit, and nothing else of the pools
 changes."""
+import types
+
 import pytest
 import torch
 
@@ -169,6 +171,9 @@ def test_torch_rotates_what_autograd_tracks(gpu):
 
 def test_kernel_takes_the_usual_rows(gpu, monkeypatch):
     """Which calls the kernel serves: torch's fallback gives the same rows, so only the count tells."""
+    _lib.load()
+    native = _lib.FAST.rope_rows
+    monkeypatch.setattr(_lib, "FAST", None)
     taken, write = [], paged.PagedKV._write_rotated
     monkeypatch.setattr(paged.PagedKV, "_write_rotated", lambda *a: taken.append(write(*a)) or taken[-1])
     inv = workloads.inv_freq()
@@ -178,6 +183,18 @@ def test_kernel_takes_the_usual_rows(gpu, monkeypatch):
         cache.append(0, [x] * 2, [x] * 2, inv_freq=inv)
     cache.append(0, [x.float()] * 2, [x] * 2, inv_freq=inv)
     assert taken == [True, True, True, False, False]
+    del taken[:]
+    monkeypatch.setattr(paged.PagedKV, "_write_rotated", write)
+    monkeypatch.setattr(_lib, "FAST", types.SimpleNamespace(rope_rows=lambda *a: taken.append(native(*a)) or taken[-1]))
+    inv = inv.to(gpu)
+    x = forms("tokens first", 1, 1, 2, 7, torch.float16, gpu)
+    bad = forms("misaligned", 1, 1, 2, 7, torch.float16, gpu)
+    for k, f in ((x, inv), (x[0], inv), (bad, inv), (x.float(), inv), (x, inv.cpu()), (x, inv.double())):
+        cache.append(0, [k] * 2, [x] * 2, inv_freq=f)
+        cache.table.prune(0, 20, cache.length(), 0)
+    assert taken == [True, True, None, None, None, None]
+    cache.append(0, [x, x.transpose(1, 2).contiguous().transpose(1, 2)], [x] * 2, inv_freq=inv)  # strides that differ
+    assert taken[-1] is None or x.transpose(1, 2).is_contiguous()
 
 
 def test_rotation_and_prune_agree(gpu):

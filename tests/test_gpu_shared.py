@@ -183,11 +183,21 @@ class Forked:
             close(out[i], *definition(q[i], r[0, layer], r[1, layer]))
 
 
-@pytest.fixture
-def calls(monkeypatch):
-    """Which decode calls read the prefix once."""
-    taken, run = [], paged.PagedKV._attend_shared
-    monkeypatch.setattr(paged.PagedKV, "_attend_shared", lambda self, *a: taken.append(1) or run(self, *a))
+@pytest.fixture(params=["native", "Python"])
+def calls(request, monkeypatch):
+    """Which decode calls read the prefix once, through either path of the wrappers."""
+    _lib.load()
+    if request.param == "Python":
+        monkeypatch.setattr(_lib, "FAST", None)
+    taken, tables = [], paged.PagedKV.shared_tables
+
+    def watched(self):
+        found = tables(self)
+        if found is not None:
+            taken.append(1)
+        return found
+
+    monkeypatch.setattr(paged.PagedKV, "shared_tables", watched)
     return taken
 
 

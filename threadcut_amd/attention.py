@@ -109,6 +109,19 @@ def _windowed(query, key, value, pending, scaling, window, sinks):
     b, hq, q, d = query.shape
     hkv, n = key.shape[1], key.shape[2]
     g = hq // hkv
+    fast = _lib.FAST
+    if q == 1 and fast is not None and query.is_cuda:
+        stream = _lib.raw_stream(query.get_device())
+        if pending is None:
+            out = fast.decode(query, key, value, scaling, stream, window, sinks)
+        else:
+            out = fast.decode_append(query, pending.kbuf, pending.vbuf, *pending.pending,
+                                     pending.n if pending.device_pos is None else pending.device_pos, scaling, stream,
+                                     window, sinks)
+        if out is not None:
+            if pending is not None:
+                pending.pending = None
+            return out
     if q == 1 and decode_supports(query, key, value):
         out = torch.empty((b, 1, hq, d), dtype=query.dtype, device=query.device)
         qg, og = query.reshape(b, hkv, g, d), out.view(b, hkv, g, d)

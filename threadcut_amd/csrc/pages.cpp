@@ -54,13 +54,8 @@ std::vector<int64_t> pages_of(const int64_t* frags, int64_t num_frags) {
   return p;
 }
 
-}  // namespace
-
-extern "C" {
-
-int64_t tc_page_tiles(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t first_pos, int32_t* tiles,
-                      int64_t max_tiles) {
-  if (malformed(frags, num_frags, page_tokens) || first_pos < 0 || max_tiles < 0) return -TC_ERR_INVALID_ARGUMENT;
+// tc_page_tiles of a well-formed list.
+int64_t tiles_of(const int64_t* frags, int64_t num_frags, int64_t first_pos, int32_t* tiles, int64_t max_tiles) {
   int64_t n = 0;
   for (int64_t i = 0; i < num_frags; ++i) {
     const int64_t s = frags[3 * i + 1], e = s + frags[3 * i + 2];
@@ -82,6 +77,34 @@ int64_t tc_page_tiles(const int64_t* frags, int64_t num_frags, int64_t page_toke
     }
   }
   return n;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t tc_page_tiles(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t first_pos, int32_t* tiles,
+                      int64_t max_tiles) {
+  if (malformed(frags, num_frags, page_tokens) || first_pos < 0 || max_tiles < 0) return -TC_ERR_INVALID_ARGUMENT;
+  return tiles_of(frags, num_frags, first_pos, tiles, max_tiles);
+}
+
+int64_t tc_page_window_tiles(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t window,
+                             int64_t sink_tokens, int32_t* tiles, int64_t max_tiles) {
+  if (malformed(frags, num_frags, page_tokens) || window < 1 || sink_tokens < 0 || max_tiles < 0)
+    return -TC_ERR_INVALID_ARGUMENT;
+  int64_t n = 0;
+  for (int64_t i = 0; i < num_frags; ++i) n += frags[3 * i + 2];
+  const int64_t first = n > window ? n - window : 0;  // the window's first token
+  if (first <= sink_tokens) return tiles_of(frags, num_frags, 0, tiles, max_tiles);
+  std::vector<int64_t> head, rest;
+  cut(frags, num_frags, 0, sink_tokens, head);
+  cut(frags, num_frags, first, n, rest);
+  const int64_t a = tiles_of(head.data(), head.size() / 3, 0, tiles, max_tiles);
+  if (a < 0) return a;
+  const bool room = tiles && a <= max_tiles;
+  const int64_t b = tiles_of(rest.data(), rest.size() / 3, first, room ? tiles + 4 * a : nullptr, max_tiles - a);
+  return b < 0 ? b : a + b;
 }
 
 int tc_page_prune(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t a, int64_t c0, int64_t c,

@@ -262,6 +262,11 @@ def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lens=None, out=N
     0..N) count, or all. The prefix is read once for the whole batch. Returns
     out [B,Hkv,G,D] (a new tensor unless given). Enqueued on the current stream.
     """
+    if _lib.FAST is not None and q.is_cuda:
+        # The whole call in native code; None for what it does not take (then as below).
+        done = _lib.FAST.decode_shared(q, k_prefix, v_prefix, k, v, lens, out, scale, _lib.raw_stream(q.get_device()))
+        if done is not None:
+            return done if out is None else out
     _check_qkv(q, k, v, "decode_attention_shared")
     _lib.require_gpu(k_prefix, v_prefix, what="decode_attention_shared")
     b, hkv, g, d = q.shape

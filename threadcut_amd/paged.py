@@ -122,6 +122,17 @@ def _tiles(frags, page_tokens, first_pos=0):
     return out
 
 
+def _window_tiles(frags, page_tokens, window, sink_tokens):
+    """_tiles of the fragments' last `window` tokens and first `sink_tokens` (tc_page_window_tiles)."""
+    f, fp, nf = _frag_arg(frags)
+    most = (min(window, 1 << 29) + min(sink_tokens, 1 << 29)) // TILE + 2 * nf + 4
+    out = np.empty((min(most, nf * (page_tokens // TILE + 2)), 4), dtype=np.int32)
+    n = _lib.load().tc_page_window_tiles(fp, nf, int(page_tokens), window, sink_tokens, _addr(out), len(out))
+    if n < 0 or n > len(out):
+        _lib.check(-n if n < 0 else _lib.TC_ERR_INVALID_ARGUMENT, "tc_page_window_tiles")
+    return out[:n]
+
+
 def tiles_of(frags, page_tokens):
     """Tile entries (page, first slot, rows) of a fragment array of pages of page_tokens
     slots, int32 [T, 3]: each fragment is cut at multiples of 16 slots, so full tiles are
@@ -177,9 +188,10 @@ class PageTable:
         """Slots that sequence b's next tokens find on its last page (none on a shared one: the others' tokens are,
         or will be, behind its own)."""
         fr = self.frags[b]
-        if len(fr) == 0 or int(fr[-1, 0]) in self.users:
+        if len(fr) == 0:
             return 0
-        return int(self.page_tokens - fr[-1, 1] - fr[-1, 2])
+        page, first, count = fr[-1].tolist()
+        return 0 if page in self.users else self.page_tokens - first - count
 
     def _drop(self, pages):
         """Takes one user from each of `pages`; returns those that nobody uses any more."""
@@ -216,6 +228,15 @@ class PageTable:
         P = self.page_tokens
         fr = self.frags[b]
         room = self._room(b)
+        if 0 < n <= room:  # the usual step: behind the last token
+            page, first, count = fr[-1].tolist()
+            self.frags[b] = fr = fr.copy()
+            fr[-1, 2] = count + n
+            self.version += 1
+            out = np.empty((n, 2), dtype=np.int64)
+            out[:, 0] = page
+            out[:, 1] = np.arange(first + count, first + count + n)
+            return out
         take = min(n, room)
         rest = n - take
         k = -(-rest // P)
@@ -245,6 +266,11 @@ class PageTable:
         n = self.length(b)
         if not (0 <= a <= c0 and c >= 0 and c0 + c <= n):
             raise ValueError(f"prune: split (a={a}, c0={c0}, c={c}) outside a sequence of {n} tokens")
+        if c == 0 and len(old) and n - int(old[-1, 2]) < a:  # last tokens of the last fragment go: it keeps its page
+            self.frags[b] = old = old.copy()
+            old[-1, 2] -= n - a
+            self.version += 1
+            return _EMPTY.copy(), []
         f, fp, nf = _frag_arg(old)
         # One buffer: kept (nf + 1 rows), suffix (nf rows), freed (nf), counts (3).
         buf = np.empty(7 * nf + 6, dtype=np.int64)
@@ -275,19 +301,14 @@ class PageTable:
         i = np.arange(len(rep)) - np.repeat(np.cumsum(fr[:, 2]) - fr[:, 2], fr[:, 2])
         return np.stack([fr[rep, 0], fr[rep, 1] + i], axis=1)
 
-    def visible(self, b, window, sink_tokens):
-        """The fragments of sequence b's last `window` tokens and its first `sink_tokens`."""
-        n = self.length(b)
-        if n - window <= sink_tokens:
-            return self.frags[b]
-        return np.concatenate([_cut(self.frags[b], 0, sink_tokens), _cut(self.frags[b], n - window, n)])
-
     def tile_table(self, window=None, sink_tokens=0):
         """int32 [B, max_tiles, 4] and tiles int32 [B] (numpy): entries {page, first slot,
-        rows, first logical position} in logical order. With a window, of the visible tokens
-        (positions then count those)."""
-        frags = self.frags if window is None else [self.visible(b, window, sink_tokens) for b in range(self.batch)]
-        per = [_tiles(f, self.page_tokens) for f in frags]
+        rows, first logical position} in logical order. With a window, of each sequence's last
+        `window` tokens and its first `sink_tokens`."""
+        if window is None:
+            per = [_tiles(f, self.page_tokens) for f in self.frags]
+        else:
+            per = [_window_tiles(f, self.page_tokens, window, sink_tokens) for f in self.frags]
         mt = max(1, max(len(t) for t in per))
         tab = np.zeros((self.batch, mt, 4), dtype=np.int32)
         cnt = np.zeros(self.batch, dtype=np.int32)
@@ -372,8 +393,11 @@ class PagedKV:
         if n == 0:
             return
         if inv_freq is not None and self.layers:
-            ks, vs = [_as_batch(t) for t in ks], [_as_batch(t) for t in vs]
             at = _to_device(_placed(slots, start)[None], self.device)
+            if _lib.FAST is not None and _lib.FAST.rope_rows(
+                    ks, vs, self.k_pools, self.v_pools, at, inv_freq, None, _lib.raw_stream(self.device.index)):
+                return
+            ks, vs = [_as_batch(t) for t in ks], [_as_batch(t) for t in vs]
             if self._write_rotated(range(self.layers), ks, vs, at, inv_freq):
                 return
             ks = [_rotated(t.reshape(1, self.kv_heads, n, HEAD_DIM), at[..., 2], inv_freq) for t in ks]
@@ -644,6 +668,18 @@ class PagedKV:
         pools' dtype; returns out [B, Hkv, G, D]. Enqueued on the current stream.
         """
         self._refuse_during_step("decode", layer)
+        fast = _lib.FAST
+        if fast is not None and split is None and q.is_cuda and 0 <= layer < self.layers:
+            # The whole call in native code; None for what it does not take (then as below).
+            tables = self.shared_tables() if window is None else None
+            pools, stream = (self.k_pools[layer], self.v_pools[layer]), _lib.raw_stream(self.device.index)
+            if tables is not None:
+                done = fast.paged_shared(q, *pools, *tables, None, None, out, scale, stream)
+            else:
+                done = fast.paged_decode(q, *pools, *self.window_table(window, sink_tokens, "decode")[:2], out, scale,
+                                         stream)
+            if done is not None:
+                return done
         _lib.require_gpu(q, what="PagedKV.decode")
         b, hkv, g, d = q.shape
         if b != self.table.batch or hkv != self.kv_heads or d != HEAD_DIM or q.dtype != self.dtype:
@@ -693,6 +729,12 @@ class PagedKV:
         # (table version, layers not written yet, tokens, the slots and their copy for each stream)
         self._step = (self.table.version, set(range(self.layers)), int(n), np.stack(slots), {})
 
+    def _step_slots(self, step):
+        """The reserved step's slots on the device (int32 [B, n, 4])."""
+        if torch.cuda.is_current_stream_capturing():  # (a replay would write this step's slots again)
+            raise RuntimeError("PagedKV.write_step: rotated rows are not captured; decode_append_at is")
+        return _lib.per_stream(step[4], self.device.index, lambda: _to_device(step[3], self.device))
+
     def write_step(self, layer, k_new, v_new, inv_freq=None, query=None):
         """The unfused order of a step: write one layer's new K/V rows ([B, Hkv, n, D], or
         [B, Hkv, D] of one token) into the slots reserve_step(n) took. Once a layer's rows
@@ -705,6 +747,13 @@ class PagedKV:
         step = getattr(self, "_step", None)
         if step is None or step[0] != self.table.version or layer not in step[1]:
             raise RuntimeError(f"PagedKV.write_step: layer {layer} has no reserved slot in this step")
+        if inv_freq is not None and _lib.FAST is not None and k_new.is_cuda:
+            # The whole call in native code; None for what it does not take (then as below).
+            done = _lib.FAST.rope_rows((k_new,), (v_new,), (self.k_pools[layer],), (self.v_pools[layer],),
+                                       self._step_slots(step), inv_freq, query, _lib.raw_stream(self.device.index))
+            if done is not None:
+                step[1].discard(layer)
+                return None if done is True else done
         b, n = self.table.batch, step[2]
         kn = k_new.reshape(b, self.kv_heads, n, HEAD_DIM)
         vn = v_new.reshape(b, self.kv_heads, n, HEAD_DIM)
@@ -720,9 +769,7 @@ class PagedKV:
                                  f"expected [{b}, Hq, {n}, {HEAD_DIM}] {self.dtype} on {self.device}")
         done = False
         if inv_freq is not None:
-            if torch.cuda.is_current_stream_capturing():  # (a replay would write this step's slots again)
-                raise RuntimeError("PagedKV.write_step: rotated rows are not captured; decode_append_at is")
-            at = _lib.per_stream(step[4], self.device.index, lambda: _to_device(step[3], self.device))
+            at = self._step_slots(step)
             if query is not None:
                 out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
             done = self._write_rotated([layer], [kn], [vn], at, inv_freq, *(([query], [out]) if query is not None else ()))
@@ -749,11 +796,17 @@ class PagedKV:
         if step is not None and step[2] != 1 and step[0] == self.table.version:
             raise RuntimeError(f"PagedKV.decode_append: the step has {step[2]} tokens a sequence (write_step takes them)")
         if (fast is not None and split is None and q.is_cuda and step is not None and step[0] == self.table.version
-                and layer in step[1] and not self.table.users):
+                and layer in step[1]):
             # The whole call in native code; None for what it does not take (then as below).
-            tab, cnt, _ = self.window_table(window, sink_tokens, "decode_append")
-            done = fast.paged_append(q, self.k_pools[layer], self.v_pools[layer], tab, cnt, k_new, v_new, out, scale,
-                                     _lib.raw_stream(q.get_device()))
+            tables = self.shared_tables() if window is None else None
+            stream = _lib.raw_stream(q.get_device())
+            if tables is not None:
+                done = fast.paged_shared(q, self.k_pools[layer], self.v_pools[layer], *tables, k_new, v_new, out, scale,
+                                         stream)
+            else:
+                tab, cnt, _ = self.window_table(window, sink_tokens, "decode_append")
+                done = fast.paged_append(q, self.k_pools[layer], self.v_pools[layer], tab, cnt, k_new, v_new, out,
+                                         scale, stream)
             if done is not None:
                 step[1].discard(layer)
                 return done
@@ -840,14 +893,14 @@ class PagedKV:
         freed page ids."""
         self._refuse_during_step("prune")
         gap = s.c0 - s.a
-        if gap and self.table.users:
+        if gap and s.c and self.table.users:
             kept = _cut(self.table.frags[b], s.c0, s.c0 + s.c)[:, 0].tolist()
             if any(p in self.table.users for p in kept):
                 raise RuntimeError(f"PagedKV.prune: tokens [{s.c0}, {s.c0 + s.c}) of sequence {b} would move, and other "
                                    "sequences share their pages")
         suffix, freed = self.table.prune(b, s.a, s.c0, s.c)
-        tiles = tiles_of(suffix, self.table.page_tokens)
-        if gap and len(tiles):
+        if gap and len(suffix):
+            tiles = tiles_of(suffix, self.table.page_tokens)
             t = np.zeros((len(tiles), 4), dtype=np.int32)
             t[:, :3] = tiles
             td = _to_device(t, self.device)
