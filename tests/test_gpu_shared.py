@@ -24,24 +24,29 @@ def definition(q, k, v):
     return torch.bmm(w, v.double()), torch.bmm(w, v.double().abs())
 
 
-def close(got, want, spread):
-    """Rounded once (eps / 2), the rest in fp32: weights to 2^-16, sums and merges far below 2^-14 of the spread."""
+def close(got, want, spread, columns):
+    """Rounded once (eps / 2), the rest in fp32: weights to 2^-16, sums and merges far below 2^-14 of the spread. More
+    than 32 query rows a KV head: the prefix's weights are rounded to the type (eps / 2 of each), in the sum over v and
+    in the one that divides it."""
     f = torch.finfo(got.dtype)
     bound = f.eps / 2 * want.abs() + 2.0 ** -14 * spread + f.smallest_normal
+    if columns > 32:
+        bound = bound * (1 + f.eps) + f.eps / 2 * (spread + want.abs())
     off = (got.double() - want).abs()
     assert torch.all(off <= bound), f"worst {(off / bound).max().item():.3g} of the bound"
 
 
 def check(out, q, kp, vp, k, v, lens):
     for i, n in enumerate(lens):
-        close(out[i], *definition(q[i], torch.cat((kp, k[i, :, :n]), 1), torch.cat((vp, v[i, :, :n]), 1)))
+        close(out[i], *definition(q[i], torch.cat((kp, k[i, :, :n]), 1), torch.cat((vp, v[i, :, :n]), 1)),
+              q.shape[0] * q.shape[2])
 
 
 CASES = [  # batch, kv heads, group, prefix, own tokens (one number: all of them)
     (4, 8, 4, 2000, [200, 1, 57, 16]), (2, 8, 1, 1, [3, 0]), (16, 8, 4, 500, [33] * 16), (3, 8, 8, 4097, [0, 0, 0]),
     (64, 2, 8, 700, list(range(64))), (5, 3, 3, 31, [17, 400, 0, 5, 64]), (1, 8, 4, 1000, [100]), (33, 1, 1, 17, [2] * 33),
     (2, 8, 4, 20000, [1000, 30]), (65, 4, 2, 15, [16] * 65), (8, 8, 2, 16, [300] * 8), (9, 8, 7, 333, [12] * 9),
-    (4, 64, 2, 600, [40] * 4), (300, 2, 4, 100, [7] * 300), (2, 1, 4, 40000, [100, 100])]
+    (4, 64, 2, 600, [40] * 4), (13, 8, 4, 900, [9] * 13), (17, 4, 8, 2500, [3] * 17), (40, 2, 8, 1200, [0] * 40), (300, 2, 4, 100, [7] * 300), (2, 1, 4, 40000, [100, 100])]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -180,7 +185,7 @@ class Forked:
 
     def check(self, out, q, layer):
         for i, r in enumerate(self.rows):
-            close(out[i], *definition(q[i], r[0, layer], r[1, layer]))
+            close(out[i], *definition(q[i], r[0, layer], r[1, layer]), q.shape[0] * q.shape[2])
 
 
 @pytest.fixture(params=["native", "Python"])
@@ -347,4 +352,4 @@ def test_bad_tiles_count_as_empty(gpu):
     k = torch.cat((pool[0, :, :16], pool[3, :, 16:], pool[2, :, 31:]), 1)
     v = torch.cat((vpool[0, :, :16], vpool[3, :, 16:], vpool[2, :, 31:]), 1)
     for i in range(3):
-        close(out[i], *definition(q[i], k, v))
+        close(out[i], *definition(q[i], k, v), 12)

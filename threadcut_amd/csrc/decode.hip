@@ -1388,7 +1388,9 @@ int shared_impl(const void* q_dev, const int64_t q_strides[3], const Prefix& x, 
   a.batch = batch;
   a.splits = Sp;
   a.part_splits = Sp + S;
-  a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  // (A scale of 0 as one so small that every weight is 1: a hidden key's -inf times it stays -inf.)
+  a.c = std::max(static_cast<float>(fabs(static_cast<double>(scale)) * 1.4426950408889634), 1e-30f);
+  a.sign = scale < 0.f ? 0x80008000u : 0u;
   if ((rc = hip_status(launch_prefix(a, dtype, static_cast<hipStream_t>(stream)), "prefix pass launch")) != TC_OK) return rc;
   return tc_decode_combine(o_part, lse_part, batch, kv_heads, group, head_dim, Sp + S, out_dev, out_strides, dtype,
                            stream);

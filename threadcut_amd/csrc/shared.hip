@@ -27,89 +27,107 @@
 namespace tc {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kStepTiles = 2;  // 16-token tiles of a wave's step
-
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// One product of 32 tokens (or dims): A and B hold 8 elements a lane.
-template <int DT>
-__device__ __forceinline__ f32x4 mma32(const uint4& a, const uint4& b, const f32x4& c) {
-  return DecodeMma<DT>::qk(a, b, c);
-}
+constexpr int kRowBytes = 2 * kHeadDim;  // a K or V row in LDS
+constexpr int kStep = 32;                // keys of a wave's step: two 16-key tiles
+constexpr int kMergeRow = kHeadDim + 16; // floats of a column's row in the merge (padded: the stores spread over the banks)
 
-struct Step {
-  uint4 k[kStepTiles][4], v[kStepTiles][4];
-  int32_t rows[kStepTiles];
+// Work-groups of W waves: CG column groups of 16 R columns, W / CG key groups.
+// Columns of all groups see every key of a work-group's tile; with one column
+// group the waves split its keys and need no barrier.
+template <int W_, int CG_, int R_>
+struct Shape {
+  static constexpr int W = W_, CG = CG_, R = R_, KG = W_ / CG_;
+  static constexpr int kColumns = 16 * R * CG;
+  static constexpr int kTiles = 2 * KG > 4 ? 2 * KG : 4;   // 16-key tiles of a work-group's tile
+  static constexpr int kSteps = kTiles / (2 * KG);         // steps of a wave in it
+  static constexpr int kBuf = 16 * kTiles * kRowBytes;     // bytes of its K (and V)
+  static constexpr bool kResidue = CG == 1;                // weights as two numbers of the type
 };
 
-// R: blocks of 16 columns a work-group holds.
-template <int DT, bool PAGED, int R>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))) void prefix_partial_kernel(
+// Slot of 16-byte chunk x of row r: the 16 rows of one chunk that a K read
+// covers, and the 8 rows of two chunks that half of a V read does, fall on
+// distinct banks.
+__device__ __forceinline__ int slot_of(int x, int r) { return x ^ (2 * (r & 7) + (r >> 3 & 1)); }
+
+template <int DT, bool PAGED, class S>
+__global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W / 4))) void prefix_partial_kernel(
     const PrefixArgs a) {
   using M = DecodeMma<DT>;
   using E = Elem<DT>;
-  __shared__ union {
-    uint32_t v[kWaves][kStepTiles][kVTileWords];
-    float acc[kWaves][16][kHeadDim + 16];
-  } s;
-  __shared__ float s_m[16][kWaves], s_l[16][kWaves];
+  constexpr int R = S::R, CG = S::CG, KG = S::KG;
+  __shared__ __attribute__((aligned(1024))) char s_k0[S::kBuf], s_k1[S::kBuf], s_v0[S::kBuf], s_v1[S::kBuf];
+  __shared__ float s_m[S::W][16], s_l[S::W][16];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
+  const int cg = wave % CG, kg = wave / CG;
   // Grid (heads, splits, column blocks), the KV head fastest: with 8 heads a head's work-groups share an XCD's L2.
   const int h = blockIdx.x, split = blockIdx.y;
-  const int c0 = static_cast<int>(blockIdx.z) * 16 * R;
+  const int c0 = static_cast<int>(blockIdx.z) * S::kColumns + 16 * R * cg;
   const int columns = a.batch * a.group;
   const char* kslab = reinterpret_cast<const char*>(a.k + h * a.sk_h);
   const char* vslab = reinterpret_cast<const char*>(a.v + h * a.sv_h);
   const int32_t row_k = static_cast<int32_t>(a.sk_t) * 2, row_v = static_cast<int32_t>(a.sv_t) * 2;
-  const int32_t steps = (a.tiles + kStepTiles - 1) / kStepTiles;
-  const int32_t stride = a.splits * kWaves;
-  int32_t st = split * kWaves + wave;
 
-  int32_t koff[4], voff[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    koff[i] = n * row_k + 64 * i + 16 * g;
-    voff[i] = (4 * g + i) * row_v + 16 * n;
-  }
-  auto load = [&](Step& x, int32_t step) {
-#pragma unroll
-    for (int t = 0; t < kStepTiles; ++t) {
-      const int32_t tile = kStepTiles * step + t;
-      const char *kp = kslab, *vp = vslab;
-      int32_t rows = 0;
-      if constexpr (PAGED) {
-        if (tile < a.tiles) {
-          const int32_t* e = a.tile_tab + 4 * static_cast<int64_t>(tile);
-          const int32_t page = const_load(e), slot = const_load(e + 1), cnt = const_load(e + 2);
-          if (!(page < 0 || page >= a.pages || slot < 0 || cnt < 0 || cnt > 16 || slot > a.page_tokens - cnt)) {
-            rows = cnt;
-            kp += page * a.sk_p * 2 + static_cast<int64_t>(slot) * row_k;
-            vp += page * a.sv_p * 2 + static_cast<int64_t>(slot) * row_v;
-          }
-        }
-      } else {
-        rows = min(max(a.n - kWaveIter * tile, 0), kWaveIter);
-        if (rows > 0) {
-          kp += static_cast<int64_t>(kWaveIter * tile) * row_k;
-          vp += static_cast<int64_t>(kWaveIter * tile) * row_v;
-        }
-      }
-      rows = __builtin_amdgcn_readfirstlane(rows);
-      x.rows[t] = rows;
-      const __amdgpu_buffer_rsrc_t rk = make_rsrc(kp, rows * row_k), rv = make_rsrc(vp, rows * row_v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x.k[t][j] = bload16(rk, koff[j]);
-        x.v[t][j] = bload16(rv, voff[j]);
+  // The work-group's tiles: groups of kTiles 16-key tiles, every splits-th of them. A wave loads the K and V of a
+  // share of the group (with one column group that of its own keys) and multiplies the two tiles of each of its steps.
+  constexpr int kParts = 4 * S::kTiles / S::W;  // pieces of 4 rows of K, and of V, that a wave loads
+  const int32_t groups = (a.tiles + S::kTiles - 1) / S::kTiles;
+
+  // Paged: lane i holds the table entry of tile i % kTiles of the (i / kTiles)-th group from `held` on.
+  int32_t e_page = 0, e_slot = 0, e_rows = 0, held = 0;
+  constexpr int kHeld = 64 / S::kTiles;
+  auto hold = [&](int32_t it) {
+    held = it;
+    const int32_t group = split + (it + lane / S::kTiles) * a.splits;
+    const int64_t tile = static_cast<int64_t>(group) * S::kTiles + lane % S::kTiles;
+    e_page = e_slot = e_rows = 0;
+    if (tile < a.tiles) {
+      const int4 e = *reinterpret_cast<const int4*>(a.tile_tab + 4 * tile);
+      // An entry outside the pool or past the page's end counts as empty.
+      if (!(e.x < 0 || e.x >= a.pages || e.y < 0 || e.z < 0 || e.z > 16 || e.y > a.page_tokens - e.z)) {
+        e_page = e.x; e_slot = e.y; e_rows = e.z;
       }
     }
   };
-  Step x[2];
-  load(x[0], st);
+  // Rows of tile t of the work-group's it-th group.
+  auto rows_of = [&](int32_t it, int t) -> int32_t {
+    if constexpr (PAGED) return __builtin_amdgcn_readlane(e_rows, (it - held) * S::kTiles + t);
+    // (i32 min and max select a vector instruction: without readfirstlane the buffer ranges would not be scalar.)
+    return __builtin_amdgcn_readfirstlane(min(max(a.n - 16 * ((split + it * a.splits) * S::kTiles + t), 0), 16));
+  };
+  // This wave's loads of group it, straight into LDS: 4 rows an instruction, lane l filling slot l % 16 of row l / 16.
+  auto load = [&](char* dk, char* dv, int32_t it) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int part = wave * kParts + i, t = part >> 2;
+      const int32_t rows = rows_of(it, t);
+      const char *kp = kslab, *vp = vslab;
+      if constexpr (PAGED) {
+        const int at = (it - held) * S::kTiles + t;
+        const int64_t page = __builtin_amdgcn_readlane(e_page, at), slot = __builtin_amdgcn_readlane(e_slot, at);
+        kp += page * a.sk_p * 2 + slot * row_k;
+        vp += page * a.sv_p * 2 + slot * row_v;
+      } else {
+        const int64_t tile = rows > 0 ? (split + it * a.splits) * S::kTiles + t : 0;
+        kp += 16 * tile * row_k;
+        vp += 16 * tile * row_v;
+      }
+      const __amdgpu_buffer_rsrc_t rk = make_rsrc(kp, rows * row_k), rv = make_rsrc(vp, rows * row_v);
+      const int r = 4 * (part & 3) + g;
+      const int x = 16 * slot_of(n, r);  // (the swizzle is its own inverse)
+      __attribute__((address_space(3))) void* pk = (__attribute__((address_space(3))) void*)(dk + 4 * part * kRowBytes);
+      __attribute__((address_space(3))) void* pv = (__attribute__((address_space(3))) void*)(dv + 4 * part * kRowBytes);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, pk, 16, r * row_k + x, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, pv, 16, r * row_v + x, 0, 0, 0);
+    }
+  };
+  const int32_t its = split < groups ? (groups - split + a.splits - 1) / a.splits : 0;
+  if constexpr (PAGED) hold(0);
+  if (its > 0) load(s_k0, s_v0, 0);
 
   uint4 qb[R][4];
 #pragma unroll
@@ -118,7 +136,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))
     const uint32_t b = static_cast<uint32_t>(c) / a.group, i = c - b * a.group;
     const uint16_t* q = a.q + b * a.sq_b + h * a.sq_h + i * a.sq_g + 8 * g;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) qb[r][j] = c < columns ? *reinterpret_cast<const uint4*>(q + 32 * j) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) {
+      qb[r][j] = c < columns ? *reinterpret_cast<const uint4*>(q + 32 * j) : make_uint4(0, 0, 0, 0);
+      qb[r][j].x ^= a.sign; qb[r][j].y ^= a.sign; qb[r][j].z ^= a.sign; qb[r][j].w ^= a.sign;
+    }
   }
 
   f32x4 acc[R][8];
@@ -130,149 +151,229 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))
 #pragma unroll
     for (int bm = 0; bm < 8; ++bm) acc[r][bm] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  // Byte offsets, in a 16-row tile, of the lane's K reads (row n, chunk 4 i + g) and its transposing V reads (row
+  // 4 g + n / 4, 8 bytes at dim 16 bm + 4 (n % 4)).
+  int koff[4], voff[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) koff[i] = n * kRowBytes + 16 * slot_of(4 * i + g, n);
+  {
+    const int r = 4 * g + (n >> 2);
+#pragma unroll
+    for (int bm = 0; bm < 8; ++bm) voff[bm] = r * kRowBytes + 16 * slot_of(2 * bm + ((n & 3) >> 1), r) + 8 * (n & 1);
+  }
 
-  char* const vl = reinterpret_cast<char*>(s.v[wave]);
-  auto step = [&](const Step& y) {
-    // V into LDS, row-major: lane (g, n) stores tokens 4g + j, dims 8n .. 8n + 7 of each tile.
+  // One step: 32 keys from (lk, lv) of which the first tile holds rows0, the second rows1. One branch, and products
+  // next to independent vector work: a compute unit runs one wave a SIMD here, so nothing else fills the gaps.
+  auto step = [&](const char* lk, const char* lv, int32_t rows0, int32_t rows1) {
+    // Rows past a tile's end score -inf from the start (their keys read as zeros).
+    f32x4 none[2];
 #pragma unroll
-    for (int t = 0; t < kStepTiles; ++t)
+    for (int j = 0; j < 4; ++j) {
+      none[0][j] = 4 * g + j < rows0 ? 0.f : neg_inf();
+      none[1][j] = 4 * g + j < rows1 ? 0.f : neg_inf();
+    }
+    uint4 kf[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(vl + (16 * t + 4 * g + j) * kVRowBytes + 16 * n) = y.v[t][j];
-    uint4 ph[R], pl[R];
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kf[t][i] = *reinterpret_cast<const uint4*>(lk + 16 * kRowBytes * t + koff[i]);
+    f32x4 sc[R][2];
+    float tmax[R];
+    bool any = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float sc[8];
 #pragma unroll
-      for (int t = 0; t < kStepTiles; ++t) {
-        f32x4 s0 = mma32<DT>(y.k[t][0], qb[r][0], f32x4{0.f, 0.f, 0.f, 0.f});
-        f32x4 s1 = mma32<DT>(y.k[t][1], qb[r][1], f32x4{0.f, 0.f, 0.f, 0.f});
-        s0 = mma32<DT>(y.k[t][2], qb[r][2], s0);
-        s1 = mma32<DT>(y.k[t][3], qb[r][3], s1);
+      for (int t = 0; t < 2; ++t) {
+        sc[r][t] = M::qk(kf[t][0], qb[r][0], none[t]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sc[4 * t + j] = 4 * g + j < y.rows[t] ? (s0[j] + s1[j]) * a.scale_log2 : neg_inf();
+        for (int i = 1; i < 4; ++i) sc[r][t] = M::qk(kf[t][i], qb[r][i], sc[r][t]);
       }
-      float mx = sc[0];
+    }
 #pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, sc[j]);
-      const float tmax = rows_max(mx);
-      // The running maximum moves only when the step's exceeds it by 2^8.
-      const float mn = (tmax > m[r] + kLazyMax || m[r] == neg_inf()) ? tmax : m[r];
-      const float ms = mn == neg_inf() ? 0.f : mn;
-      if (__any(mn != m[r] && m[r] != neg_inf())) {
-        const float alpha = __builtin_amdgcn_exp2f(m[r] - ms);
+    for (int r = 0; r < R; ++r) {
+      const f32x4 &x = sc[r][0], &y = sc[r][1];
+      tmax[r] = a.c * rows_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                     fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
+      any |= tmax[r] > m[r] + kLazyMax;
+    }
+    // The running maximum (of scores times c > 0) moves only when the step's exceeds it by 2^8.
+    if (__any(any)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool move = tmax[r] > m[r] + kLazyMax;
+        const float alpha = move ? __builtin_amdgcn_exp2f(m[r] - tmax[r]) : 1.f;  // 0 while nothing was seen
+        m[r] = move ? tmax[r] : m[r];
 #pragma unroll
         for (int bm = 0; bm < 8; ++bm) acc[r][bm] *= alpha;
         l[r] *= alpha;
       }
-      m[r] = mn;
-      float p[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(sc[j] - ms);
-      l[r] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-      // The weights as two numbers of the type (the second what rounding the first left), as in the decode kernel.
-      uint32_t w[4], e[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = M::pack(p[2 * j], p[2 * j + 1]);
-        e[j] = M::pack(p[2 * j] - E::lo(w[j]), p[2 * j + 1] - E::hi(w[j]));
-      }
-      ph[r] = make_uint4(w[0], w[1], w[2], w[3]);
-      pl[r] = make_uint4(e[0], e[1], e[2], e[3]);
     }
+    // V^T[16 bm + n][4g .. 4g + 3 of both tiles], once for all column blocks.
+    uint4 vf[8];
 #pragma unroll
     for (int bm = 0; bm < 8; ++bm) {
-      // V^T[16 bm + n][4g .. 4g + 3 of both tiles], by the transposing read (decode.hip).
-      uint2 t2[kStepTiles];
+      uint2 t2[2];
 #pragma unroll
-      for (int t = 0; t < kStepTiles; ++t)
+      for (int t = 0; t < 2; ++t)
         t2[t] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) lds_s4*)(vl + (16 * t + 4 * g + (n >> 2)) * kVRowBytes + 32 * bm +
-                                                        8 * (n & 3))));
-      const uint4 av = make_uint4(t2[0].x, t2[0].y, t2[1].x, t2[1].y);
+            (__attribute__((address_space(3))) lds_s4*)(lv + 16 * kRowBytes * t + voff[bm])));
+      vf[bm] = make_uint4(t2[0].x, t2[0].y, t2[1].x, t2[1].y);
+    }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        acc[r][bm] = mma32<DT>(av, ph[r], acc[r][bm]);
-        acc[r][bm] = mma32<DT>(av, pl[r], acc[r][bm]);
+    for (int r = 0; r < R; ++r) {
+      const float ms = m[r] == neg_inf() ? 0.f : m[r];
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(sc[r][j >> 2][j & 3], a.c, -ms));
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = M::pack(p[2 * j], p[2 * j + 1]);
+      const uint4 ph = make_uint4(w[0], w[1], w[2], w[3]);
+      if constexpr (S::kResidue) {
+        // What rounding to the type left of the weights goes through the product too, as in the decode kernel.
+        l[r] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        uint32_t e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = M::pack(p[2 * j] - E::lo(w[j]), p[2 * j + 1] - E::hi(w[j]));
+        const uint4 pl = make_uint4(e[0], e[1], e[2], e[3]);
+#pragma unroll
+        for (int bm = 0; bm < 8; ++bm) {
+          acc[r][bm] = M::qk(vf[bm], ph, acc[r][bm]);
+          acc[r][bm] = M::qk(vf[bm], pl, acc[r][bm]);
+        }
+      } else {
+        // Many columns are bound by the products: weights rounded to the type once, in the sum too, as in prefill.
+        constexpr uint32_t kOnes = DT == TC_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[r] = E::dot2(w[j], kOnes, l[r]);
+#pragma unroll
+        for (int bm = 0; bm < 8; ++bm) acc[r][bm] = M::qk(vf[bm], ph, acc[r][bm]);
       }
     }
   };
 
-  // Two steps in flight; no load past the wave's last.
-  if (st < steps) {
-    for (;;) {
-      load(x[1], st + stride);
-      step(x[0]);
-      load(x[0], st + 2 * stride);
-      if (st + stride < steps) step(x[1]);
-      st += 2 * stride;
-      if (st >= steps) break;
+  // A group from (lk, lv) while the next one loads into (dk, dv).
+  auto body = [&](int32_t it, const char* lk, const char* lv, char* dk, char* dv) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of group it have landed
+    if constexpr (CG > 1) __syncthreads();               // and everyone's; (dk, dv) is read no more
+    int32_t rows[2 * S::kSteps];
+#pragma unroll
+    for (int i = 0; i < 2 * S::kSteps; ++i) rows[i] = rows_of(it, 2 * S::kSteps * kg + i);
+    if (it + 1 < its) {
+      if constexpr (PAGED)
+        if (it + 1 - held >= kHeld) hold(it + 1);
+      load(dk, dv, it + 1);
     }
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) {
+      const int at = (S::kSteps * kg + i) * kStep * kRowBytes;
+      step(lk + at, lv + at, rows[2 * i], rows[2 * i + 1]);
+    }
+  };
+  for (int32_t it = 0; it < its; it += 2) {
+    body(it, s_k0, s_v0, s_k1, s_v1);
+    if (it + 1 < its) body(it + 1, s_k1, s_v1, s_k0, s_v0);
   }
 
-  // The four waves' results merged block by block through LDS.
+  // The key groups' results of a column are merged block by block through LDS and written by the first group. Lane
+  // (g, n) holds dims 16 bm + 4 g .. + 3 of column n.
+  constexpr int kHold = S::kBuf / (16 * kMergeRow * 4);  // waves' rows that a tile buffer holds
+  static_assert((KG - 1) * CG <= 4 * kHold, "the other groups' rows fit the tile buffers");
+  auto rows16 = [&](int w) {  // of wave w >= CG
+    const int i = w - CG, buf = i / kHold;
+    return reinterpret_cast<float*>(buf == 0 ? s_k0 : buf == 1 ? s_k1 : buf == 2 ? s_v0 : s_v1) + i % kHold * 16 * kMergeRow;
+  };
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    __syncthreads();  // the V tiles, or the block before, are done with
+    float L = rows_sum(l[r]), mx = m[r];
+    if constexpr (KG > 1) {
+      __syncthreads();  // the tiles, or the block before, are done with
+      if (kg > 0) {
+#pragma unroll
+        for (int bm = 0; bm < 8; ++bm)
+          *reinterpret_cast<float4*>(rows16(wave) + n * kMergeRow + 16 * bm + 4 * g) =
+              make_float4(acc[r][bm][0], acc[r][bm][1], acc[r][bm][2], acc[r][bm][3]);
+      }
+      if (g == 0) { s_m[wave][n] = mx; s_l[wave][n] = L; }
+      __syncthreads();
+      if (kg > 0) continue;
+#pragma unroll
+      for (int k = 1; k < KG; ++k) mx = fmaxf(mx, s_m[k * CG + cg][n]);
+      const float ms = mx == neg_inf() ? 0.f : mx;
+      const float mine = __builtin_amdgcn_exp2f(m[r] - ms);
+      L *= mine;
+#pragma unroll
+      for (int bm = 0; bm < 8; ++bm) acc[r][bm] *= mine;
+#pragma unroll
+      for (int k = 1; k < KG; ++k) {
+        const float f = __builtin_amdgcn_exp2f(s_m[k * CG + cg][n] - ms);
+        L += s_l[k * CG + cg][n] * f;
+#pragma unroll
+        for (int bm = 0; bm < 8; ++bm) {
+          const float4 o = *reinterpret_cast<const float4*>(rows16(k * CG + cg) + n * kMergeRow + 16 * bm + 4 * g);
+          acc[r][bm][0] += o.x * f;
+          acc[r][bm][1] += o.y * f;
+          acc[r][bm][2] += o.z * f;
+          acc[r][bm][3] += o.w * f;
+        }
+      }
+    }
+    const int c = c0 + 16 * r + n;
+    if (c >= columns) continue;
+    const float inv = L == 0.f ? 0.f : __builtin_amdgcn_rcpf(L);
+    const uint32_t b = static_cast<uint32_t>(c) / a.group, i = c - b * a.group;
+    const int64_t part = ((static_cast<int64_t>(b) * a.heads + h) * a.part_splits + split) * a.group + i;
+    float* const o = a.o_part + part * kHeadDim + 4 * g;
 #pragma unroll
     for (int bm = 0; bm < 8; ++bm)
-      *reinterpret_cast<float4*>(&s.acc[wave][n][16 * bm + 4 * g]) =
-          make_float4(acc[r][bm][0], acc[r][bm][1], acc[r][bm][2], acc[r][bm][3]);
-    const float lr = rows_sum(l[r]);
-    if (g == 0) { s_m[n][wave] = m[r]; s_l[n][wave] = lr; }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < 16 * (kHeadDim / 2); idx += 64 * kWaves) {
-      const int col = idx / (kHeadDim / 2), d = 2 * (idx % (kHeadDim / 2));
-      const int c = c0 + 16 * r + col;
-      if (c >= columns) break;
-      float mx = neg_inf();
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, s_m[col][w]);
-      const float ms = mx == neg_inf() ? 0.f : mx;
-      float L = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(s_m[col][w] - ms);
-        const float2 o = *reinterpret_cast<const float2*>(&s.acc[w][col][d]);
-        L += s_l[col][w] * f;
-        o0 += o.x * f;
-        o1 += o.y * f;
-      }
-      const float inv = L == 0.f ? 0.f : __builtin_amdgcn_rcpf(L);
-      const uint32_t b = static_cast<uint32_t>(c) / a.group, i = c - b * a.group;
-      const int64_t part = ((static_cast<int64_t>(b) * a.heads + h) * a.part_splits + split) * a.group + i;
-      *reinterpret_cast<float2*>(a.o_part + part * kHeadDim + d) = make_float2(o0 * inv, o1 * inv);
-      if (d == 0) a.lse_part[part] = L == 0.f ? neg_inf() : (mx + __builtin_amdgcn_logf(L)) * kLn2;
-    }
+      *reinterpret_cast<float4*>(o + 16 * bm) =
+          make_float4(acc[r][bm][0] * inv, acc[r][bm][1] * inv, acc[r][bm][2] * inv, acc[r][bm][3] * inv);
+    if (g == 0) a.lse_part[part] = L == 0.f ? neg_inf() : (mx + __builtin_amdgcn_logf(L)) * kLn2;
   }
 }
 
-// Blocks of 16 columns a work-group holds: all, up to four.
-int column_blocks(int batch, int group) {
+// The shape of a call: all columns in one work-group up to 256, else in blocks of them.
+struct Plan {
+  int cg, r, tiles;
+  int64_t blocks;
+};
+
+Plan shape_plan(int batch, int group) {
   const int64_t c = static_cast<int64_t>(batch) * group;
-  return c <= 16 ? 1 : c <= 32 ? 2 : 4;
+  if (c <= 16) return Plan{1, 1, 8, 1};
+  if (c <= 32) return Plan{1, 2, 8, 1};
+  const int cg = c <= 64 ? 2 : c <= 128 ? 4 : 8;
+  return Plan{cg, 2, cg == 2 ? 8 : 4, ceil_div(c, 256)};
+}
+
+template <int DT, bool PAGED, int W, int CG, int R>
+void launch_shape(const PrefixArgs& a, int64_t blocks, hipStream_t s) {
+  using S = Shape<W, CG, R>;
+  hipLaunchKernelGGL((prefix_partial_kernel<DT, PAGED, S>), dim3(a.heads, a.splits, static_cast<unsigned>(blocks)),
+                     dim3(64 * W), 0, s, a);
 }
 
 template <int DT, bool PAGED>
 void launch(const PrefixArgs& a, hipStream_t s) {
-  const int r = column_blocks(a.batch, a.group);
-  const dim3 grid(a.heads, a.splits, (a.batch * a.group + 16 * r - 1) / (16 * r)), block(64 * kWaves);
-  if (r == 1)
-    hipLaunchKernelGGL((prefix_partial_kernel<DT, PAGED, 1>), grid, block, 0, s, a);
-  else if (r == 2)
-    hipLaunchKernelGGL((prefix_partial_kernel<DT, PAGED, 2>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((prefix_partial_kernel<DT, PAGED, 4>), grid, block, 0, s, a);
+  const Plan p = shape_plan(a.batch, a.group);
+  switch (p.cg) {
+    case 1:
+      if (p.r == 1) return launch_shape<DT, PAGED, 4, 1, 1>(a, p.blocks, s);
+      return launch_shape<DT, PAGED, 4, 1, 2>(a, p.blocks, s);
+    case 2: return launch_shape<DT, PAGED, 8, 2, 2>(a, p.blocks, s);
+    case 4: return launch_shape<DT, PAGED, 8, 4, 2>(a, p.blocks, s);
+    default: return launch_shape<DT, PAGED, 8, 8, 2>(a, p.blocks, s);
+  }
 }
 
 }  // namespace
 
-// As many work-groups as compute units, but a step for every wave.
+// As many work-groups as compute units (one fits a unit), but a group of tiles for every one.
 int prefix_splits(int batch, int heads, int group, int64_t tiles, int cus) {
-  const int64_t r = column_blocks(batch, group);
-  const int64_t per_split = heads * ((static_cast<int64_t>(batch) * group + 16 * r - 1) / (16 * r));
-  const int64_t most = ceil_div(ceil_div(tiles, kStepTiles), kWaves);
-  return static_cast<int>(std::max<int64_t>(tiles > 0, std::min<int64_t>({(cus + per_split / 2) / per_split, most, 1024})));
+  const Plan p = shape_plan(batch, group);
+  const int64_t per_split = heads * p.blocks;
+  const int64_t most = ceil_div(tiles, p.tiles);
+  return static_cast<int>(std::max<int64_t>(tiles > 0, std::min<int64_t>({cus / per_split, most, 1024})));
 }
 
 hipError_t launch_prefix(const PrefixArgs& a, int dtype, hipStream_t stream) {

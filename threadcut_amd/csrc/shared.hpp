@@ -21,7 +21,8 @@ struct PrefixArgs {
   int32_t pages, page_tokens;
   int heads, group, batch;
   int splits, part_splits;
-  float scale_log2;
+  float c;                  // |scale| log2(e), > 0
+  uint32_t sign;            // 0x80008000 for a negative scale: flips the queries
 };
 
 // Splits of the prefix pass for `tiles` tiles, and the launch itself.
