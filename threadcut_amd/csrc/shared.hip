@@ -40,16 +40,18 @@ template <int W_, int CG_, int R_>
 struct Shape {
   static constexpr int W = W_, CG = CG_, R = R_, KG = W_ / CG_;
   static constexpr int kColumns = 16 * R * CG;
-  static constexpr int kTiles = 2 * KG > 4 ? 2 * KG : 4;   // 16-key tiles of a work-group's tile
+  static constexpr int kTiles = 8;                         // 16-key tiles of a work-group's tile
   static constexpr int kSteps = kTiles / (2 * KG);         // steps of a wave in it
   static constexpr int kBuf = 16 * kTiles * kRowBytes;     // bytes of its K (and V)
   static constexpr bool kResidue = CG == 1;                // weights as two numbers of the type
 };
 
-// Slot of 16-byte chunk x of row r: the 16 rows of one chunk that a K read
-// covers, and the 8 rows of two chunks that half of a V read does, fall on
+// Slot of 16-byte chunk x of row r of a 16-key tile. Half of a V read covers 8
+// rows of two neighbouring chunks, a quarter of a K read rows 0-3 and 12-15 of
+// one chunk and rows 4-11 of its neighbour (which the hardware takes together:
+// with 2 (r % 8) + r / 8 every K read met two rows a bank); both fall on
 // distinct banks.
-__device__ __forceinline__ int slot_of(int x, int r) { return x ^ (2 * (r & 7) + (r >> 3 & 1)); }
+__device__ __forceinline__ int slot_of(int x, int r) { return x ^ (2 * ((r & 7) ^ (r >> 3 << 2)) + (r >> 3)); }
 
 template <int DT, bool PAGED, class S>
 __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W / 4))) void prefix_partial_kernel(
@@ -142,12 +144,15 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
     }
   }
 
-  f32x4 acc[R][8];
-  float m[R], l[R];
+  // acc: O^T; l: the sum of the weights, in every register (a product with ones); m: the running maximum, in units of
+  // a.c times a score, -inf at first, and ms what is subtracted (0 then).
+  f32x4 acc[R][8], l[R];
+  float m[R], ms[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     m[r] = neg_inf();
-    l[r] = 0.f;
+    ms[r] = 0.f;
+    l[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int bm = 0; bm < 8; ++bm) acc[r][bm] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -162,9 +167,19 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
     for (int bm = 0; bm < 8; ++bm) voff[bm] = r * kRowBytes + 16 * slot_of(2 * bm + ((n & 3) >> 1), r) + 8 * (n & 1);
   }
 
-  // One step: 32 keys from (lk, lv) of which the first tile holds rows0, the second rows1. One branch, and products
-  // next to independent vector work: a compute unit runs one wave a SIMD here, so nothing else fills the gaps.
-  auto step = [&](const char* lk, const char* lv, int32_t rows0, int32_t rows1) {
+  // One step: 32 keys from (lk, lv); rows0 and rows1 of them in the two tiles. Vector instructions are
+  // what many columns are bound by (the exponentials alone take as long as half of the products), so the rest of the
+  // softmax is kept short: the maximum is compared with the running one lane by lane, and reduced over the lanes only
+  // where some lane's exceeds it; the weights are summed by the matrix core.
+  uint4 kf[2][4];
+  auto read_k = [&](const char* lk) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kf[t][i] = *reinterpret_cast<const uint4*>(lk + 16 * kRowBytes * t + koff[i]);
+  };
+  // kf holds the step's K; `more`: the next step's is read from lk_next under the products with V.
+  auto step = [&](const char* lk_next, const char* lv, bool more, int32_t rows0, int32_t rows1) {
     // Rows past a tile's end score -inf from the start (their keys read as zeros).
     f32x4 none[2];
 #pragma unroll
@@ -172,14 +187,7 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
       none[0][j] = 4 * g + j < rows0 ? 0.f : neg_inf();
       none[1][j] = 4 * g + j < rows1 ? 0.f : neg_inf();
     }
-    uint4 kf[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) kf[t][i] = *reinterpret_cast<const uint4*>(lk + 16 * kRowBytes * t + koff[i]);
     f32x4 sc[R][2];
-    float tmax[R];
-    bool any = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -189,26 +197,7 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
         for (int i = 1; i < 4; ++i) sc[r][t] = M::qk(kf[t][i], qb[r][i], sc[r][t]);
       }
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const f32x4 &x = sc[r][0], &y = sc[r][1];
-      tmax[r] = a.c * rows_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                     fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
-      any |= tmax[r] > m[r] + kLazyMax;
-    }
-    // The running maximum (of scores times c > 0) moves only when the step's exceeds it by 2^8.
-    if (__any(any)) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool move = tmax[r] > m[r] + kLazyMax;
-        const float alpha = move ? __builtin_amdgcn_exp2f(m[r] - tmax[r]) : 1.f;  // 0 while nothing was seen
-        m[r] = move ? tmax[r] : m[r];
-#pragma unroll
-        for (int bm = 0; bm < 8; ++bm) acc[r][bm] *= alpha;
-        l[r] *= alpha;
-      }
-    }
-    // V^T[16 bm + n][4g .. 4g + 3 of both tiles], once for all column blocks.
+    // V^T[16 bm + n][4g .. 4g + 3 of both tiles], once for all column blocks; read under the softmax.
     uint4 vf[8];
 #pragma unroll
     for (int bm = 0; bm < 8; ++bm) {
@@ -219,35 +208,60 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
             (__attribute__((address_space(3))) lds_s4*)(lv + 16 * kRowBytes * t + voff[bm])));
       vf[bm] = make_uint4(t2[0].x, t2[0].y, t2[1].x, t2[1].y);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    float mx[R];
+    bool any = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float ms = m[r] == neg_inf() ? 0.f : m[r];
+      const f32x4 &x = sc[r][0], &y = sc[r][1];
+      mx[r] = a.c * fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+      any |= mx[r] > m[r] + kLazyMax;
+    }
+    // The running maximum moves only when the step's exceeds it by 2^8, for a column's lanes together.
+    if (__any(any)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float tmax = rows_max(mx[r]);
+        const bool move = tmax > m[r] + kLazyMax;
+        const float alpha = move ? __builtin_amdgcn_exp2f(m[r] - tmax) : 1.f;  // 0 while nothing was seen
+        m[r] = move ? tmax : m[r];
+        ms[r] = m[r] == neg_inf() ? 0.f : m[r];
+#pragma unroll
+        for (int bm = 0; bm < 8; ++bm) acc[r][bm] *= alpha;
+        l[r] *= alpha;
+      }
+    }
+    uint4 ph[R], pl[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       float p[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(sc[r][j >> 2][j & 3], a.c, -ms));
-      uint32_t w[4];
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(sc[r][j >> 2][j & 3], a.c, -ms[r]));
+      uint32_t w[4], e[4] = {};
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = M::pack(p[2 * j], p[2 * j + 1]);
-      const uint4 ph = make_uint4(w[0], w[1], w[2], w[3]);
       if constexpr (S::kResidue) {
-        // What rounding to the type left of the weights goes through the product too, as in the decode kernel.
-        l[r] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        uint32_t e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = M::pack(p[2 * j] - E::lo(w[j]), p[2 * j + 1] - E::hi(w[j]));
-        const uint4 pl = make_uint4(e[0], e[1], e[2], e[3]);
+      }
+      ph[r] = make_uint4(w[0], w[1], w[2], w[3]);
+      pl[r] = make_uint4(e[0], e[1], e[2], e[3]);
+    }
+    if (more) read_k(lk_next);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int bm = 0; bm < 8; ++bm) {
-          acc[r][bm] = M::qk(vf[bm], ph, acc[r][bm]);
-          acc[r][bm] = M::qk(vf[bm], pl, acc[r][bm]);
-        }
-      } else {
-        // Many columns are bound by the products: weights rounded to the type once, in the sum too, as in prefill.
-        constexpr uint32_t kOnes = DT == TC_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
+    for (int r = 0; r < R; ++r) {
+      constexpr uint32_t kOnes = DT == TC_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
+      const uint4 ones = make_uint4(kOnes, kOnes, kOnes, kOnes);
+      l[r] = M::qk(ones, ph[r], l[r]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) l[r] = E::dot2(w[j], kOnes, l[r]);
+      for (int bm = 0; bm < 8; ++bm) acc[r][bm] = M::qk(vf[bm], ph[r], acc[r][bm]);
+      if constexpr (S::kResidue) {
+        // What rounding to the type left of the weights goes through the product too, as in the decode kernel (with
+        // many columns, which are bound by the products, it does not, as in prefill).
+        l[r] = M::qk(ones, pl[r], l[r]);
 #pragma unroll
-        for (int bm = 0; bm < 8; ++bm) acc[r][bm] = M::qk(vf[bm], ph, acc[r][bm]);
+        for (int bm = 0; bm < 8; ++bm) acc[r][bm] = M::qk(vf[bm], pl[r], acc[r][bm]);
       }
     }
   };
@@ -264,11 +278,12 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
         if (it + 1 - held >= kHeld) hold(it + 1);
       load(dk, dv, it + 1);
     }
+    const int at = S::kSteps * kg * kStep * kRowBytes;
+    read_k(lk + at);
 #pragma unroll
-    for (int i = 0; i < S::kSteps; ++i) {
-      const int at = (S::kSteps * kg + i) * kStep * kRowBytes;
-      step(lk + at, lv + at, rows[2 * i], rows[2 * i + 1]);
-    }
+    for (int i = 0; i < S::kSteps; ++i)
+      step(lk + at + (i + 1) * kStep * kRowBytes, lv + at + i * kStep * kRowBytes, i + 1 < S::kSteps, rows[2 * i],
+           rows[2 * i + 1]);
   };
   for (int32_t it = 0; it < its; it += 2) {
     body(it, s_k0, s_v0, s_k1, s_v1);
@@ -285,7 +300,7 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
   };
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float L = rows_sum(l[r]), mx = m[r];
+    float L = l[r][0], mx = m[r];
     if constexpr (KG > 1) {
       __syncthreads();  // the tiles, or the block before, are done with
       if (kg > 0) {
@@ -334,16 +349,16 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
 
 // The shape of a call: all columns in one work-group up to 256, else in blocks of them.
 struct Plan {
-  int cg, r, tiles;
+  int cg, r;
   int64_t blocks;
 };
 
 Plan shape_plan(int batch, int group) {
   const int64_t c = static_cast<int64_t>(batch) * group;
-  if (c <= 16) return Plan{1, 1, 8, 1};
-  if (c <= 32) return Plan{1, 2, 8, 1};
+  if (c <= 16) return Plan{1, 1, 1};
+  if (c <= 32) return Plan{1, 2, 1};
   const int cg = c <= 64 ? 2 : c <= 128 ? 4 : 8;
-  return Plan{cg, 2, cg == 2 ? 8 : 4, ceil_div(c, 256)};
+  return Plan{cg, 2, ceil_div(c, 256)};
 }
 
 template <int DT, bool PAGED, int W, int CG, int R>
@@ -372,7 +387,7 @@ void launch(const PrefixArgs& a, hipStream_t s) {
 int prefix_splits(int batch, int heads, int group, int64_t tiles, int cus) {
   const Plan p = shape_plan(batch, group);
   const int64_t per_split = heads * p.blocks;
-  const int64_t most = ceil_div(tiles, p.tiles);
+  const int64_t most = ceil_div(tiles, 8);
   return static_cast<int>(std::max<int64_t>(tiles > 0, std::min<int64_t>({cus / per_split, most, 1024})));
 }
 
