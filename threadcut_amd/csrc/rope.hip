@@ -118,13 +118,30 @@ int check_strides(const char* what, const int64_t* st) {
 }
 
 template <int LAYERS, int HEADS>
-void launch(const RopeArgs<LAYERS>& a, int dtype, int layers, hipStream_t s) {
+void launch_heads(const RopeArgs<LAYERS>& a, int dtype, int layers, hipStream_t s) {
   const dim3 grid((a.total + kTileRows - 1) / kTileRows,
                   2 * ((a.kv_heads + HEADS - 1) / HEADS) + (a.q_heads + HEADS - 1) / HEADS, layers);
   if (dtype == TC_DTYPE_F16)
     hipLaunchKernelGGL((rope_rows_kernel<TC_DTYPE_F16, LAYERS, HEADS>), grid, dim3(kThreads), 0, s, a);
   else
     hipLaunchKernelGGL((rope_rows_kernel<TC_DTYPE_BF16, LAYERS, HEADS>), grid, dim3(kThreads), 0, s, a);
+}
+
+// Heads a thread takes: with more, its angles serve more rows and more of its
+// loads are in flight, with fewer there are more work-groups. By the rows of
+// all heads and layers (us with 1, 2, 4 and 8 heads, 8 KV and 32 query heads):
+// 48 (one token) 3.40, 3.67, 4.17, 4.94; 1584 3.39, 3.61, 4.20, 5.19; 28800
+// 5.77, 5.18, 5.22, 6.29; 67200 9.50, 7.98, 7.71, 8.61; 98304 11.6, 10.4, 8.30,
+// 10.2; 2.5 million (24 layers, no queries) 228, 223, 228, 229.
+template <int LAYERS>
+void launch(const RopeArgs<LAYERS>& a, int dtype, int layers, hipStream_t s) {
+  const int64_t rows = static_cast<int64_t>(a.total) * (2 * a.kv_heads + a.q_heads) * layers;
+  if (rows <= 6000)
+    launch_heads<LAYERS, 1>(a, dtype, layers, s);
+  else if (rows <= 50000)
+    launch_heads<LAYERS, 2>(a, dtype, layers, s);
+  else
+    launch_heads<LAYERS, 4>(a, dtype, layers, s);
 }
 
 }  // namespace
@@ -208,14 +225,14 @@ extern "C" int tc_paged_append_rope(const void* const* k_rows_host, const int64_
   if (num_layers == 1) {
     RopeArgs<1> a;
     fill(a, 0, 1);
-    launch<1, 8>(a, dtype, 1, s);
+    launch(a, dtype, 1, s);
     return hip_status(hipGetLastError(), "rotated row write launch");
   }
   for (int l0 = 0; l0 < num_layers; l0 += kMaxLayers) {
     RopeArgs<kMaxLayers> a;
     const int nl = num_layers - l0 < kMaxLayers ? num_layers - l0 : kMaxLayers;
     fill(a, l0, nl);
-    launch<kMaxLayers, 8>(a, dtype, nl, s);
+    launch(a, dtype, nl, s);
     if ((rc = hip_status(hipGetLastError(), "rotated row write launch")) != TC_OK) return rc;
   }
   return TC_OK;
