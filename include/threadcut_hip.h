@@ -614,11 +614,15 @@ int tc_match_split(const int64_t* cached, int64_t n_cached, const int64_t* fresh
 int64_t tc_page_tiles(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t first_pos, int32_t* tiles,
                       int64_t max_tiles);
 
-/* The same for a sliding window: the tiles of the last `window` tokens and of
- * the first sink_tokens (each with its logical start), which is the key set of
- * the newest token's query. window >= 1, sink_tokens >= 0. */
-int64_t tc_page_window_tiles(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t window,
-                             int64_t sink_tokens, int32_t* tiles, int64_t max_tiles);
+/* The tile table of `batch` sequences (frags[b]: num_frags[b] fragments, the
+ * first at logical position first_pos): row b of table [batch, pitch, 4] gets
+ * its entries, the rest of the row zeros, and tiles[b] their number. window >
+ * 0: of its last `window` tokens and its first sink_tokens, which is the key
+ * set of the newest token's query. Returns the largest number of a sequence;
+ * with table NULL nothing is written, and a pitch below it is refused. */
+int64_t tc_page_table(const int64_t* const* frags, const int64_t* num_frags, int64_t batch,
+                      int64_t page_tokens, int64_t first_pos, int64_t window, int64_t sink_tokens,
+                      int32_t* table, int64_t pitch, int32_t* tiles);
 
 /* Prune of one sequence: keep logical tokens [0, a) and [c0, c0 + c). kept
  * (room for num_frags + 1 rows) receives the new fragment list, the two kept

@@ -3,6 +3,7 @@ appends, on the CPU."""
 import ctypes
 import random
 
+import numpy as np
 import pytest
 
 from threadcut_amd import _lib
@@ -118,21 +119,47 @@ def test_rotated_append_validation():
     assert _placed([[4, 1], [5, 0]], 7).tolist() == [[4, 1, 7, 0], [5, 0, 8, 0]]
 
 
-def test_shared_tiles():
+def test_shared_fragments():
     t = PageTable(40, 16, batch=3)
     t.reserve(0, 70)
     t.fork(0, 1, 70)
     t.fork(0, 2, 40)
     t.reserve(2, 5)
-    assert t.shared_tiles(*t.tile_table()) == 2  # the third tile has 16 rows in two sequences, 8 in the third
+    assert t.shared_frags() == 2  # the third page has 16 tokens in two sequences, 8 in the third
     t.release(2)
-    assert t.shared_tiles(*t.tile_table()) == 0
+    assert t.shared_frags() == 0
     t.fork(1, 2, 70)
-    assert t.shared_tiles(*t.tile_table()) == 5
+    assert t.shared_frags() == 5
+    whole, counts = t.tile_table()
+    own, none = t.tile_table(skip=5)
+    assert own.shape == (3, 0, 4) and none.tolist() == [0, 0, 0]
+    for b, n in enumerate((1, 20, 33)):
+        t.reserve(b, n)
+    assert t.shared_frags() == 5
+    head, _ = t.tile_table()
+    own, mine = t.tile_table(skip=5)
+    assert mine.tolist() == [1, 2, 3]
     for b in range(3):
-        t.reserve(b, 1)
-    assert t.shared_tiles(*t.tile_table()) == 5
-    assert PageTable(4, 16).shared_tiles(*PageTable(4, 16).tile_table()) == 0
+        assert head[b, :5].tolist() == whole[b, :5].tolist()
+        assert own[b, :mine[b]].tolist() == head[b, 5:5 + mine[b]].tolist()
+    assert PageTable(4, 16).shared_frags() == 0
+
+
+def test_table_refusals():
+    f = _lib.load().tc_page_table
+    frags = np.array([[3, 0, 10], [5, 4, 30]], dtype=np.int64)
+    args = np.array([frags.__array_interface__["data"][0], 2], dtype=np.int64)
+    base = args.__array_interface__["data"][0]
+    tab, cnt = np.zeros((1, 4, 4), dtype=np.int32), np.zeros(1, dtype=np.int32)
+    ptr = lambda a: a.__array_interface__["data"][0]
+    call = lambda P=64, first=0, w=0, s=0, t=None, pitch=0, c=None, b=1: f(base, base + 8, b, P, first, w, s, t, pitch, c)
+    # Token 5 of 40 (slot 5 of page 3) and token 20 (slot 14 of page 5) begin a tile of their own behind the sinks'.
+    assert call() == 4 and call(w=1) == 1 and call(w=35, s=2) == 5 and call(w=20, s=1) == 4
+    assert call(P=32) == call(first=-1) == call(w=-1) == call(s=-1) == call(b=0) == -_lib.TC_ERR_INVALID_ARGUMENT
+    assert call(t=ptr(tab), pitch=3) == -_lib.TC_ERR_INVALID_ARGUMENT  # no counts
+    assert call(t=ptr(tab), pitch=3, c=ptr(cnt)) == -_lib.TC_ERR_INVALID_ARGUMENT  # four tiles
+    assert call(w=20, s=1, t=ptr(tab), pitch=4, c=ptr(cnt)) == 4
+    assert cnt.tolist() == [4] and tab[0].tolist() == [[3, 0, 1, 0], [5, 14, 2, 20], [5, 16, 16, 22], [5, 32, 2, 38]]
 
 
 def test_shared_entry_refusals():

@@ -1,5 +1,7 @@
 """Decode over a prefix that all sequences share, against the definition in float64: the contiguous entry point, forked
 sequences of a paged cache, and a run of the paged operators together."""
+import types
+
 import pytest
 import torch
 
@@ -192,18 +194,21 @@ class Forked:
 def calls(request, monkeypatch):
     """Which decode calls read the prefix once, through either path of the wrappers."""
     _lib.load()
-    if request.param == "Python":
-        monkeypatch.setattr(_lib, "FAST", None)
-    taken, tables = [], paged.PagedKV.shared_tables
+    taken = []
+    fast = types.SimpleNamespace(**{n: getattr(_lib.FAST, n) for n in dir(_lib.FAST) if n[0] != "_"})
+    shared, attend = fast.paged_shared, paged.PagedKV._attend_shared
 
-    def watched(self):
-        found = tables(self)
-        if found is not None:
+    def native(*a):
+        done = shared(*a)
+        if done is not None:
             taken.append(1)
-        return found
+        return done
 
-    monkeypatch.setattr(paged.PagedKV, "shared_tables", watched)
-    return taken
+    fast.paged_shared = native
+    monkeypatch.setattr(_lib, "FAST", fast if request.param == "native" else None)
+    monkeypatch.setattr(paged.PagedKV, "_attend_shared", lambda self, *a: taken.append(2) or attend(self, *a))
+    yield taken
+    assert set(taken) == {1 if request.param == "native" else 2}
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])

@@ -89,22 +89,44 @@ int64_t tc_page_tiles(const int64_t* frags, int64_t num_frags, int64_t page_toke
   return tiles_of(frags, num_frags, first_pos, tiles, max_tiles);
 }
 
-int64_t tc_page_window_tiles(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t window,
-                             int64_t sink_tokens, int32_t* tiles, int64_t max_tiles) {
-  if (malformed(frags, num_frags, page_tokens) || window < 1 || sink_tokens < 0 || max_tiles < 0)
+int64_t tc_page_table(const int64_t* const* frags, const int64_t* num_frags, int64_t batch, int64_t page_tokens,
+                      int64_t first_pos, int64_t window, int64_t sink_tokens, int32_t* table, int64_t pitch,
+                      int32_t* tiles) {
+  if (batch < 1 || !frags || !num_frags || first_pos < 0 || window < 0 || sink_tokens < 0 || pitch < 0 ||
+      (table && !tiles))
     return -TC_ERR_INVALID_ARGUMENT;
-  int64_t n = 0;
-  for (int64_t i = 0; i < num_frags; ++i) n += frags[3 * i + 2];
-  const int64_t first = n > window ? n - window : 0;  // the window's first token
-  if (first <= sink_tokens) return tiles_of(frags, num_frags, 0, tiles, max_tiles);
-  std::vector<int64_t> head, rest;
-  cut(frags, num_frags, 0, sink_tokens, head);
-  cut(frags, num_frags, first, n, rest);
-  const int64_t a = tiles_of(head.data(), head.size() / 3, 0, tiles, max_tiles);
-  if (a < 0) return a;
-  const bool room = tiles && a <= max_tiles;
-  const int64_t b = tiles_of(rest.data(), rest.size() / 3, first, room ? tiles + 4 * a : nullptr, max_tiles - a);
-  return b < 0 ? b : a + b;
+  int64_t most = 0;
+  std::vector<int64_t> seen;
+  for (int64_t b = 0; b < batch; ++b) {
+    if (malformed(frags[b], num_frags[b], page_tokens)) return -TC_ERR_INVALID_ARGUMENT;
+    int64_t n = 0;
+    for (int64_t i = 0; window && i < num_frags[b]; ++i) n += frags[b][3 * i + 2];
+    const int64_t first = window && n > window ? n - window : 0;  // the window's first token
+    int32_t* row = table ? table + b * pitch * 4 : nullptr;
+    int64_t count;
+    if (first <= sink_tokens) {
+      count = tiles_of(frags[b], num_frags[b], first_pos, row, pitch);
+    } else {
+      seen.clear();
+      cut(frags[b], num_frags[b], 0, sink_tokens, seen);
+      const int64_t head = static_cast<int64_t>(seen.size() / 3);
+      cut(frags[b], num_frags[b], first, n, seen);
+      count = tiles_of(seen.data(), head, first_pos, row, pitch);
+      if (count < 0) return count;
+      const bool room = row && count <= pitch;
+      const int64_t rest = tiles_of(seen.data() + 3 * head, seen.size() / 3 - head, first_pos + first,
+                                    room ? row + 4 * count : nullptr, room ? pitch - count : 0);
+      count = rest < 0 ? rest : count + rest;
+    }
+    if (count < 0) return count;
+    most = std::max(most, count);
+    if (table) {
+      if (count > pitch) return -TC_ERR_INVALID_ARGUMENT;
+      std::fill(row + 4 * count, row + 4 * pitch, 0);
+      tiles[b] = static_cast<int32_t>(count);
+    }
+  }
+  return most;
 }
 
 int tc_page_prune(const int64_t* frags, int64_t num_frags, int64_t page_tokens, int64_t a, int64_t c0, int64_t c,

@@ -76,6 +76,12 @@ def _to_device(arr, device):
     return torch.from_numpy(np.ascontiguousarray(arr)).pin_memory().to(device, non_blocking=True)
 
 
+def _upload(arrays, device):
+    """int32 arrays as device tensors, in one copy (each a multiple of 16 bytes but the last)."""
+    flat = _to_device(np.concatenate([a.ravel() for a in arrays]), device)
+    return tuple(t.view(a.shape) for t, a in zip(flat.split([a.size for a in arrays]), arrays))
+
+
 def _as_batch(t):
     """[Hkv, n, D] as [1, Hkv, n, D]."""
     return t if t.dim() == 4 else t.unsqueeze(0)
@@ -120,17 +126,6 @@ def _tiles(frags, page_tokens, first_pos=0):
         _lib.check(0 if lib.tc_page_tiles(fp, nf, int(page_tokens), int(first_pos), _addr(out), n) == n
                    else _lib.TC_ERR_INVALID_ARGUMENT, "tc_page_tiles")
     return out
-
-
-def _window_tiles(frags, page_tokens, window, sink_tokens):
-    """_tiles of the fragments' last `window` tokens and first `sink_tokens` (tc_page_window_tiles)."""
-    f, fp, nf = _frag_arg(frags)
-    most = (min(window, 1 << 29) + min(sink_tokens, 1 << 29)) // TILE + 2 * nf + 4
-    out = np.empty((min(most, nf * (page_tokens // TILE + 2)), 4), dtype=np.int32)
-    n = _lib.load().tc_page_window_tiles(fp, nf, int(page_tokens), window, sink_tokens, _addr(out), len(out))
-    if n < 0 or n > len(out):
-        _lib.check(-n if n < 0 else _lib.TC_ERR_INVALID_ARGUMENT, "tc_page_window_tiles")
-    return out[:n]
 
 
 def tiles_of(frags, page_tokens):
@@ -301,27 +296,36 @@ class PageTable:
         i = np.arange(len(rep)) - np.repeat(np.cumsum(fr[:, 2]) - fr[:, 2], fr[:, 2])
         return np.stack([fr[rep, 0], fr[rep, 1] + i], axis=1)
 
-    def tile_table(self, window=None, sink_tokens=0):
+    def tile_table(self, window=None, sink_tokens=0, skip=0):
         """int32 [B, max_tiles, 4] and tiles int32 [B] (numpy): entries {page, first slot,
         rows, first logical position} in logical order. With a window, of each sequence's last
-        `window` tokens and its first `sink_tokens`."""
-        if window is None:
-            per = [_tiles(f, self.page_tokens) for f in self.frags]
-        else:
-            per = [_window_tiles(f, self.page_tokens, window, sink_tokens) for f in self.frags]
-        mt = max(1, max(len(t) for t in per))
-        tab = np.zeros((self.batch, mt, 4), dtype=np.int32)
-        cnt = np.zeros(self.batch, dtype=np.int32)
-        for b, ts in enumerate(per):
-            tab[b, :len(ts)] = ts
-            cnt[b] = len(ts)
+        `window` tokens and its first `sink_tokens`; with `skip`, without its first `skip`
+        fragments (the same in every sequence)."""
+        lib, B = _lib.load(), self.batch
+        frags = [_frag_arg(f) for f in self.frags]
+        # One array of what the call reads: the lists' addresses, then their lengths.
+        args = np.array([a + 24 * skip for _, a, _ in frags] + [n - skip for _, _, n in frags], dtype=np.int64)
+        base = _addr(args)
+        start = int(self.frags[0][:skip, 2].sum()) if skip else 0
+        fixed = (base, base + 8 * B, B, self.page_tokens, start, min(int(window or 0), 1 << 40),
+                 min(int(sink_tokens), 1 << 40))
+        most = lib.tc_page_table(*fixed, None, 0, None)
+        tab = np.empty((B, max(1, most) if not skip else max(0, most), 4), dtype=np.int32)
+        cnt = np.empty(B, dtype=np.int32)
+        if most < 0 or lib.tc_page_table(*fixed, _addr(tab), tab.shape[1], _addr(cnt)) != most:
+            _lib.check(_lib.TC_ERR_INVALID_ARGUMENT, "tc_page_table")
         return tab, cnt
 
-    def shared_tiles(self, tab, cnt):
-        """Leading tiles of a tile_table that are the same in every sequence."""
-        most = int(cnt.min()) if self.users and self.batch > 1 else 0
-        apart = (tab[:, :most, :3] != tab[:1, :most, :3]).any(axis=(0, 2))
-        return int(apart.argmax()) if apart.any() else most
+    def shared_frags(self):
+        """Leading fragments that are the same in every sequence."""
+        if not self.users or self.batch < 2:
+            return 0
+        most = min(len(f) for f in self.frags)
+        first = self.frags[0][:most]
+        for f in self.frags[1:]:
+            apart = (f[:most] != first[:most]).any(axis=1)
+            most = int(apart.argmax()) if apart.any() else most
+        return most
 
     def token_offsets(self, page_bytes, slot_bytes, pitch=None):
         """int32 [B, pitch]: byte offset of every logical token's row within a head slab of
@@ -364,6 +368,7 @@ class PagedKV:
             "cuda", torch.cuda.current_device() if dev.index is None else dev.index)
         # (version, what device_table or device_offsets returns, for each stream)
         self._dev_table = self._dev_off = self._dev_window = self._dev_shared = (None, None)
+        self._last_tables = (None, None, None)  # what the last decode() read, and for which table, window and stream
 
     @property
     def layers(self):
@@ -502,15 +507,16 @@ class PagedKV:
             return None
         version, copies = self._dev_shared
         if version != self.table.version:
-            tab, cnt = self.table.tile_table()
-            t = self.table.shared_tiles(tab, cnt)
-            copies = (tab[0, :t], tab[:, t:], cnt - t, {}) if t * TILE >= SHARED_MIN_TOKENS else False
+            t, head = self.table.shared_frags(), self.table.frags[0]
+            copies = False
+            if t and int(head[:t, 2].sum()) >= SHARED_MIN_TOKENS:
+                copies = (_tiles(head[:t], self.table.page_tokens), *self.table.tile_table(skip=t), {})
             self._dev_shared = (self.table.version, copies)
         if copies is False:
             return None
         head, own, cnt, streams = copies
-        return (streams.get(_lib.raw_stream(self.device.index)) or _lib.per_stream(
-            streams, self.device.index, lambda: tuple(_to_device(x, self.device) for x in (head, own, cnt))))
+        return (streams.get(_lib.raw_stream(self.device.index))
+                or _lib.per_stream(streams, self.device.index, lambda: _upload((head, own, cnt), self.device)))
 
     def _attend_shared(self, tables, layer, q, k_new, v_new, scale, out):
         """decode (k_new None) or decode_append of checked tensors over shared_tables."""
@@ -551,7 +557,7 @@ class PagedKV:
 
     def _upload_table(self, window=None, sink_tokens=0):
         tab, cnt = self.table.tile_table(window, sink_tokens)
-        return _to_device(tab, self.device), _to_device(cnt, self.device), tab.shape[1]
+        return *_upload((tab, cnt), self.device), tab.shape[1]
 
     def device_offsets(self):
         """(token offsets int32 [B, pitch], pitch) on the device: the byte offset of each logical
@@ -671,12 +677,17 @@ class PagedKV:
         fast = _lib.FAST
         if fast is not None and split is None and q.is_cuda and 0 <= layer < self.layers:
             # The whole call in native code; None for what it does not take (then as below).
-            tables = self.shared_tables() if window is None else None
-            pools, stream = (self.k_pools[layer], self.v_pools[layer]), _lib.raw_stream(self.device.index)
-            if tables is not None:
-                done = fast.paged_shared(q, *pools, *tables, None, None, out, scale, stream)
+            stream = _lib.raw_stream(self.device.index)
+            key = (self.table.version, window, sink_tokens, stream)
+            if self._last_tables[0] != key:  # the layers of a step ask for the same ones
+                shared = self.shared_tables() if window is None else None
+                self._last_tables = (key, shared, None if shared else self.window_table(window, sink_tokens, "decode"))
+            _, shared, table = self._last_tables
+            if shared:
+                done = fast.paged_shared(q, self.k_pools[layer], self.v_pools[layer], *shared, None, None, out, scale,
+                                         stream)
             else:
-                done = fast.paged_decode(q, *pools, *self.window_table(window, sink_tokens, "decode")[:2], out, scale,
+                done = fast.paged_decode(q, self.k_pools[layer], self.v_pools[layer], table[0], table[1], out, scale,
                                          stream)
             if done is not None:
                 return done
