@@ -269,3 +269,17 @@ def test_step_without_native_paths(gpu, monkeypatch):
         cache.reserve_step()
         got.append((cache.write_step(0, x, x, inv_freq=inv, query=q), cache.k_pools[0], cache.v_pools[0]))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_rows_that_do_not_fit_change_nothing(gpu):
+    inv = workloads.inv_freq().to(gpu)
+    cache = paged.PagedKV(2, 2, 9, 16, device=gpu)
+    x, y = rand(1, (1, 2, 20, D), torch.float16, gpu), rand(1, (1, 2, 19, D), torch.float16, gpu)
+    cache.append(0, [x] * 2, [x] * 2, inv_freq=inv)
+    table, pools = cache.table.frags[0].copy(), [t.clone() for t in cache.k_pools + cache.v_pools]
+    free = list(cache.table.free)
+    for ks, vs in (([x, y], [x, x]), ([x, x], [x, y]), ([x, x.expand(2, 2, 20, D)], [x, x])):
+        with pytest.raises(ValueError, match="append"):
+            cache.append(0, ks, vs, inv_freq=inv)
+    assert (cache.table.frags[0] == table).all() and cache.table.free == free
+    assert all(torch.equal(a, b) for a, b in zip(cache.k_pools + cache.v_pools, pools))

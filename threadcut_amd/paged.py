@@ -220,7 +220,7 @@ class PageTable:
         """Slots of the next n tokens of sequence b, in order: int64 [n, 2] of (page, slot)."""
         if n < 0:
             raise ValueError("reserve: n must be >= 0")
-        P = self.page_tokens
+        n, P = int(n), self.page_tokens
         fr = self.frags[b]
         room = self._room(b)
         if 0 < n <= room:  # the usual step: behind the last token
@@ -237,22 +237,24 @@ class PageTable:
         k = -(-rest // P)
         if k > len(self.free):
             raise RuntimeError(f"PageTable: {k} pages needed, {len(self.free)} free")
-        parts = []
+        out = np.empty((n, 2), dtype=np.int64)
         if take:
             page, end = int(fr[-1, 0]), int(fr[-1, 1] + fr[-1, 2])
-            parts.append(np.stack([np.full(take, page), np.arange(end, end + take)], axis=1))
+            out[:take, 0] = page
+            out[:take, 1] = np.arange(end, end + take)
             fr = fr.copy()
             fr[-1, 2] += take
         if k:
-            pages = np.array([self.free.pop() for _ in range(k)], dtype=np.int64)
-            counts = np.full(k, P, dtype=np.int64)
-            counts[-1] = rest - (k - 1) * P
-            fr = np.concatenate([fr, np.stack([pages, np.zeros(k, dtype=np.int64), counts], axis=1)])
-            idx = np.arange(rest)
-            parts.append(np.stack([pages[idx // P], idx % P], axis=1))
+            more = np.zeros((k, 3), dtype=np.int64)
+            more[:, 0] = [self.free.pop() for _ in range(k)]
+            more[:, 2] = P
+            more[-1, 2] = rest - (k - 1) * P
+            fr = np.concatenate([fr, more])
+            out[take:, 0] = np.repeat(more[:, 0], more[:, 2])
+            out[take:, 1] = np.arange(rest) % P
         self.frags[b] = fr
         self.version += 1
-        return np.concatenate(parts).astype(np.int64) if parts else np.zeros((0, 2), dtype=np.int64)
+        return out
 
     def prune(self, b, a, c0, c):
         """Keep tokens [0, a) and [c0, c0 + c) of sequence b; returns (the kept
@@ -388,9 +390,9 @@ class PagedKV:
         if len(ks) != self.layers or len(vs) != self.layers:
             raise ValueError(f"append: {self.layers} layers of K and V expected")
         n = ks[0].shape[-2]
-        for t in list(ks) + list(vs):
-            if t.shape[-2] != n or t.numel() != self.kv_heads * n * HEAD_DIM:
-                raise ValueError(f"append: every layer's K and V must be [{self.kv_heads}, {n}, {HEAD_DIM}]")
+        native = inv_freq is not None and _lib.FAST is not None  # (which checks the rows itself)
+        if not native:
+            self._check_rows(ks, vs, n)
         if inv_freq is not None:
             _check_inv_freq(inv_freq, "append")
         start = self.table.length(b)
@@ -399,9 +401,15 @@ class PagedKV:
             return
         if inv_freq is not None and self.layers:
             at = _to_device(_placed(slots, start)[None], self.device)
-            if _lib.FAST is not None and _lib.FAST.rope_rows(
-                    ks, vs, self.k_pools, self.v_pools, at, inv_freq, None, _lib.raw_stream(self.device.index)):
-                return
+            if native:
+                if _lib.FAST.rope_rows(ks, vs, self.k_pools, self.v_pools, at, inv_freq, None,
+                                       _lib.raw_stream(self.device.index)):
+                    return
+                try:
+                    self._check_rows(ks, vs, n)
+                except ValueError:
+                    self.table.prune(b, start, start + n, 0)
+                    raise
             ks, vs = [_as_batch(t) for t in ks], [_as_batch(t) for t in vs]
             if self._write_rotated(range(self.layers), ks, vs, at, inv_freq):
                 return
@@ -416,6 +424,11 @@ class PagedKV:
             v = v.reshape(self.kv_heads, n, HEAD_DIM)
             kp[pages, :, sl] = k.transpose(0, 1).to(self.dtype)
             vp[pages, :, sl] = v.transpose(0, 1).to(self.dtype)
+
+    def _check_rows(self, ks, vs, n):
+        for t in list(ks) + list(vs):
+            if t.shape[-2] != n or t.numel() != self.kv_heads * n * HEAD_DIM:
+                raise ValueError(f"append: every layer's K and V must be [{self.kv_heads}, {n}, {HEAD_DIM}]")
 
     def _write_rows(self, layers, ks, vs, slots):
         """New tokens' rows, per layer [B, Hkv, n, D], into the pools' slots (int64 [B, n, 2] of (page, slot) on the
