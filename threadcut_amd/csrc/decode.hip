@@ -62,9 +62,6 @@ namespace {
 #ifndef TC_DECODE_WPE_PAGED
 #define TC_DECODE_WPE_PAGED 2  // the same for the paged instantiations
 #endif
-#ifndef TC_DECODE_STAMPS
-#define TC_DECODE_STAMPS 0  // 1: the measurement build; every partial wave records a timeline
-#endif
 
 constexpr int64_t kMaxTokens = int64_t(1) << 29;  // token positions stay 32-bit in the kernel
 constexpr int kWaves = TC_DECODE_WAVES;
@@ -78,63 +75,6 @@ constexpr int kShortWaves = 2;
 constexpr int kSplitGranule = kWaves * kWaveIter > 64 ? kWaves * kWaveIter : 64;  // split length granule
 static_assert(kSplitGranule % (kShortWaves * kWaveIter) == 0, "short plans split at the same granule");
 
-struct PartialArgs {
-  const uint16_t* q;
-  const uint16_t* k;
-  const uint16_t* v;
-  float* o_part;       // [B, H, part_splits, G, D]: this call's splits from part0 on
-  float* lse_part;     // [B, H, part_splits, G]
-  const int32_t* lens; // [B] or null
-  int64_t n;
-  int64_t sq_b, sq_h, sq_g;
-  int64_t sk_b, sk_h, sk_t;
-  int64_t sv_b, sv_h, sv_t;
-  int heads, group, splits, split_tokens;
-  int part_splits, part0;
-  int interleave;      // 0: split s owns tokens [s*T, (s+1)*T); 1: 16-token tiles dealt round-robin
-  int longest_first;   // per-sequence lengths, batch <= 64: work-group row z serves the z-th longest sequence
-  float scale_log2;    // softmax scale * log2(e)
-  // Append (k_new != null): the cache holds n - 1 tokens and the new token's
-  // K/V rows [B, H, D] are attended from k_new/v_new and written to row n - 1
-  // of the cache (k_w/v_w) by wave 0 of split 0; no other wave reads that row.
-  const uint16_t* k_new;
-  const uint16_t* v_new;
-  int64_t skn_b, skn_h, svn_b, svn_h;
-  uint16_t* k_w;
-  uint16_t* v_w;
-  // Paged cache (decode_partial_kernel<DT, true, ...>): k and v are page pools
-  // [pages, H, P, D] with element strides (sk_b, sk_h, sk_t) = (page, head,
-  // token). Sequence b's keys are the tiles tile_tab[b * max_tiles + i],
-  // i < tiles[b], each {page, first slot, rows, 0}: rows (<= 16) consecutive
-  // slots of one page. Entries outside the pool or the page count as empty.
-  const int32_t* tile_tab;
-  const int32_t* tiles;
-  int64_t max_tiles;
-  int32_t pages, page_tokens;
-  // Paged append with device lengths (tok_off != null): sequence b holds
-  // lens[b] tokens before this step; tile entries carry their first logical
-  // position in the 4th word, and a tile's rows are those below lens[b]
-  // (tiles reserved ahead read nothing). The new token goes to logical
-  // position lens[b], whose row sits tok_off[b * tok_pitch + lens[b]] bytes
-  // into the head slab of the pools.
-  const int32_t* tok_off;
-  int64_t tok_pitch;
-  // Window (decode_partial_kernel<..., true>): sequence b's query sees its last
-  // `window` tokens, an appended one among them, and the first `sinks` ones.
-  int32_t window, sinks;
-  // One split: the result itself, rounded to the element type as the combine
-  // rounds it (null: the partial goes to o_part, lse_part).
-  uint16_t* out;
-  int64_t so_b, so_h, so_g;
-#if TC_DECODE_STAMPS
-  // Per wave ((b * heads + h) * splits + split) * waves + wave, 8 words:
-  // realtime-clock stamps (100 MHz) at the kernel's start, after the first
-  // tile's step, at the loop's end, after the merge barrier and after the
-  // partial stores are issued, then HW_REG_HW_ID and HW_REG_XCC_ID.
-  unsigned long long* stamps;
-#endif
-};
-
 struct CombineArgs {
   const float* o_part;
   const float* lse_part;
@@ -143,376 +83,18 @@ struct CombineArgs {
   int heads, group, splits;
 };
 
-// APPEND: the kernel attends (and writes) the new token of an append call
-// (a.k_new != null); DIRECT: it writes the result (a.out != null), of one
-// split. WINDOW (contiguous caches, tiles dealt round-robin): only the first
-// a.sinks tokens and the last a.window are read: the tokens between the two
-// are left out of the index space that the tiles are dealt from, in which the
-// window follows the sinks' last, perhaps partial, tile. The other
-// instantiations carry none of that code.
+// Grid (heads, splits, batch), the KV head fastest: consecutive work-groups go
+// to consecutive XCDs, so with 8 KV heads every split of head h runs on XCD h
+// and its partials stay in that XCD's L2 for the combine. W waves per
+// work-group: kWaves, or kShortWaves for short caches.
 template <int DT, bool PAGED, bool APPEND, bool DIRECT, int W, bool WINDOW = false>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? TC_DECODE_WPE_PAGED : TC_DECODE_WPE))) void decode_partial_kernel(const PartialArgs a) {
-  using M = DecodeMma<DT>;
-  using E = Elem<DT>;
-  // W waves per work-group (kWaves, or kShortWaves for short caches).
   __shared__ uint32_t s_vt[W][kVTileWords];
-  // The merge's rows are padded by 16 words, so the float4 stores of the g
-  // heads (one head per 16 lanes) fall on distinct banks.
   __shared__ float s_acc[W][8][kHeadDim + 16];
   __shared__ float s_m[8][W];
   __shared__ float s_l[8][W];
-
-#if TC_DECODE_STAMPS
-  const unsigned long long st_start = __builtin_amdgcn_s_memrealtime();
-  unsigned long long st_first = 0, st_loop = 0, st_merge = 0;
-#endif
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 15;   // head column (also the token row of the K operand)
-  const int g = lane >> 4;   // lane group
-  // Grid (heads, splits, batch), the KV head fastest: consecutive work-groups
-  // go to consecutive XCDs, so with 8 KV heads every split of head h runs on
-  // XCD h and its partials stay in that XCD's L2 for the combine.
-  const int h = blockIdx.x;
-  const int split = blockIdx.y;
-  // With per-sequence lengths the work-groups of the z-th longest sequence
-  // take grid row z, so the longest sequences are dispatched first (ties by
-  // index): lane j ranks sequence j by length, and the ballot finds the lane
-  // of rank z.
-  int b = blockIdx.z;
-  int32_t len_b = 0;  // longest-first: sequence b's length, read with the others
-  if (!PAGED && a.longest_first) {
-    const int B = static_cast<int>(gridDim.z);
-    const int32_t mine = lane < B ? a.lens[lane] : 0;
-    int rank = 0;
-    for (int i = 0; i < B; ++i) {
-      const int32_t other = __builtin_amdgcn_readlane(mine, i);
-      rank += (other > mine || (other == mine && i < lane)) ? 1 : 0;
-    }
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < B && rank == static_cast<int>(blockIdx.z));
-    b = hit ? __builtin_ctzll(hit) : b;
-    len_b = __builtin_amdgcn_readlane(mine, b);
-  }
-
-  // Paged: the pools' head slabs, pages added per tile; otherwise sequence b's slabs.
-  const char* kslab = reinterpret_cast<const char*>(a.k + (PAGED ? 0 : b * a.sk_b) + h * a.sk_h);
-  const char* vslab = reinterpret_cast<const char*>(a.v + (PAGED ? 0 : b * a.sv_b) + h * a.sv_h);
-  const int32_t row_k = static_cast<int32_t>(a.sk_t) * 2, row_v = static_cast<int32_t>(a.sv_t) * 2;
-  __asm__ volatile("" ::"s"(kslab), "s"(vslab));
-  const int32_t nt = static_cast<int32_t>(a.n);
-  const int32_t len_cap = APPEND ? nt - 1 : nt;
-  // The wave's first tile and the distance between its tiles.
-  int32_t tok, tok_step, wave_tokens = 0;
-  if (a.interleave) {
-    tok = (split * W + wave) * kWaveIter;
-    tok_step = a.splits * W * kWaveIter;
-  } else {
-    wave_tokens = a.split_tokens / W;
-    tok = split * a.split_tokens + wave * wave_tokens;
-    tok_step = kWaveIter;
-  }
-  const int32_t* tab = PAGED ? a.tile_tab + static_cast<int64_t>(b) * a.max_tiles * 4 : nullptr;
-  // Paged: lane i holds the table entry of the wave's i-th tile (tiles past
-  // the 64th read theirs from memory). The entries are requested before the
-  // tile count is known, bounded by the table's row, so the two reads are in
-  // flight together.
-  int32_t e_page = 0, e_slot = 0, e_cnt = 0, e_pos = 0;
-  const int32_t ti = tok + lane * tok_step;
-  if constexpr (PAGED) {
-    if ((ti >> 4) < a.max_tiles) {
-      const int4 e = *reinterpret_cast<const int4*>(tab + 4 * (ti >> 4));
-      e_page = e.x; e_slot = e.y; e_cnt = e.z; e_pos = e.w;
-    }
-  }
-  int32_t len = len_cap;
-  int32_t last_tile = -1;  // paged append: the tile whose last row is the new token's slot
-  int32_t plen = -1;  // paged append with device lengths: tokens cached before this step
-  if constexpr (PAGED) {
-    // Token index space of 16 per tile; a tile's own row count masks the rest.
-    // The tile count and lengths are read with scalar loads (constant for the
-    // kernel's lifetime).
-    const int32_t ntiles = min(max(const_load(a.tiles + b), 0), static_cast<int32_t>(a.max_tiles));
-    len = 16 * ntiles;
-    if (a.tok_off) plen = max(const_load(a.lens + b), 0);
-    else if (APPEND)
-      last_tile = ntiles - 1;
-  } else if (a.lens) {
-    len = min(max(a.longest_first ? len_b : a.lens[b], 0), len_cap);
-  }
-  // The window's first token, and where it stands in the index space of the
-  // tiles (0: the sequence is read whole).
-  int32_t win0 = 0, win_at = 0;
-  const int32_t last = len;  // tokens in the cache
-  if constexpr (WINDOW) {
-    win0 = __builtin_amdgcn_readfirstlane(max(len + (APPEND ? 1 : 0) - a.window, 0));
-    if (win0 > a.sinks) {
-      win_at = (a.sinks + kWaveIter - 1) / kWaveIter * kWaveIter;
-      len = win_at + last - win0;
-    } else {
-      win0 = 0;
-    }
-  }
-  const int32_t end = a.interleave ? len : min(tok + wave_tokens, len);
-
-  // K: token n of the tile, bytes [64 i + 16 g, +16) for block i.
-  // V: tokens 4g + j, dims 8n .. 8n + 7.
-  int32_t koff[4], voff[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    koff[i] = n * row_k + 64 * i + 16 * g;
-    voff[i] = (4 * g + i) * row_v + 16 * n;
-  }
-  // Rows each preloaded tile contributes: none past the wave's tiles; the
-  // append's last tile less the new token's row (attended from k_new); with
-  // device lengths, the rows below lens[b].
-  int32_t e_rows = 0;
-  if constexpr (PAGED) {
-    if (ti < end) {
-      e_rows = (ti >> 4) == last_tile ? e_cnt - 1 : e_cnt;
-      if (plen >= 0) e_rows = min(e_cnt, max(plen - e_pos, 0));
-    }
-  }
-  int32_t li = 0;  // the wave's tiles loaded so far
-  auto load = [&](Tile& tl, int32_t t0) {
-    if constexpr (PAGED) {
-      int32_t page = 0, slot = 0, rows = 0;
-      if (li < 64) {
-        page = __builtin_amdgcn_readlane(e_page, li);
-        slot = __builtin_amdgcn_readlane(e_slot, li);
-        rows = __builtin_amdgcn_readlane(e_rows, li);
-      } else if (t0 < end) {
-        const int4 e = *reinterpret_cast<const int4*>(tab + 4 * (t0 >> 4));
-        page = __builtin_amdgcn_readfirstlane(e.x);
-        slot = __builtin_amdgcn_readfirstlane(e.y);
-        int32_t r = (t0 >> 4) == last_tile ? e.z - 1 : e.z;
-        if (plen >= 0) r = min(e.z, max(plen - e.w, 0));
-        rows = __builtin_amdgcn_readfirstlane(r);
-      }
-      ++li;
-      load_paged_tile(tl, kslab, vslab, row_k, row_v, a.sk_b * 2, a.sv_b * 2, a.pages, a.page_tokens, page, slot,
-                      rows, koff, voff);
-    } else if constexpr (WINDOW) {
-      const bool sink = t0 < win_at;
-      const int32_t at = sink || t0 >= end ? t0 : t0 - win_at + win0;
-      load_tile(tl, kslab, vslab, row_k, row_v, t0 < end ? at : 0, t0 >= end ? 0 : sink ? a.sinks : last, koff, voff);
-    } else {
-      load_tile(tl, kslab, vslab, row_k, row_v, t0, end, koff, voff);
-    }
-  };
-  // The index at which the keys of the tile at t0 end.
-  auto limit = [&](const Tile& tl, int32_t t0) -> int32_t {
-    if constexpr (PAGED) return t0 + tl.rows;
-    if constexpr (WINDOW) return t0 < win_at ? a.sinks : end;
-    return end;
-  };
-  Tile t[2];
-  load(t[0], tok);
-
-  // Q as the B operand: head n, dims 32 i + 8 g .. +8 (zero for n >= G).
-  uint4 qb[4];
-  {
-    const uint16_t* qrow = a.q + b * a.sq_b + h * a.sq_h + n * a.sq_g + 8 * g;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      qb[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (n < a.group) qb[i] = *reinterpret_cast<const uint4*>(qrow + 32 * i);
-    }
-  }
-
-  mfma_f4 acc[8];
-#pragma unroll
-  for (int bm = 0; bm < 8; ++bm) acc[bm] = mfma_f4{0.f, 0.f, 0.f, 0.f};
-  float m = neg_inf(), l = 0.f;
-
-  // One 16-token tile whose first token is t0 (tokens >= lim are masked).
-  auto step = [&](const Tile& tl, int32_t t0, int32_t lim) {
-    // S^T block: two independent chains of two MFMAs each.
-    mfma_f4 s0 = M::qk(tl.k[0], qb[0], mfma_f4{0.f, 0.f, 0.f, 0.f});
-    mfma_f4 s1 = M::qk(tl.k[1], qb[1], mfma_f4{0.f, 0.f, 0.f, 0.f});
-    s0 = M::qk(tl.k[2], qb[2], s0);
-    s1 = M::qk(tl.k[3], qb[3], s1);
-    // V into LDS, row-major, while the matrix core works: lane (g, n)
-    // stores tokens 4g + j, dims 8n .. 8n + 7.
-    char* vrow = reinterpret_cast<char*>(s_vt[wave]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(vrow + (4 * g + j) * kVRowBytes + 16 * n) = tl.v[j];
-    float x[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      x[r] = (t0 + 4 * g + r < lim) ? (s0[r] + s1[r]) * a.scale_log2 : neg_inf();
-    const float tmax = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-    // Lazy running maximum: moves only when the tile's exceeds it by kLazyMax.
-    const float mn = (tmax > m + kLazyMax || m == neg_inf()) ? tmax : m;
-    const float ms = (mn == neg_inf()) ? 0.f : mn;
-    // Rescale what was accumulated (nothing while m is still -inf: acc and l are zero).
-    if (__any(mn != m && m != neg_inf())) {
-      const float alpha = __builtin_amdgcn_exp2f(m - ms);  // 0 while nothing was seen
-#pragma unroll
-      for (int bm = 0; bm < 8; ++bm) acc[bm] *= alpha;
-      l *= alpha;
-    }
-    m = mn;
-    float p[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(x[r] - ms);
-    l += (p[0] + p[1]) + (p[2] + p[3]);
-    const uint32_t h01 = M::pack(p[0], p[1]), h23 = M::pack(p[2], p[3]);
-    const uint32_t r01 = M::pack(p[0] - E::lo(h01), p[1] - E::hi(h01));
-    const uint32_t r23 = M::pack(p[2] - E::lo(h23), p[3] - E::hi(h23));
-    const uint2 phi = make_uint2(h01, h23), plo = make_uint2(r01, r23);
-#pragma unroll
-    for (int bm = 0; bm < 8; ++bm) {
-      // A operand V^T[16 bm + n][4g .. 4g + 3]: ds_read_b64_tr_b16 hands lane n
-      // of a 16-lane group element (n % 4) of what lane 4 j + n / 4 addressed,
-      // for j = 0..3; lane (g, n) addresses row 4g + n / 4, dims 16 bm + 4 (n % 4).
-      const lds_s4 t4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) lds_s4*)(vrow + (4 * g + (n >> 2)) * kVRowBytes + 32 * bm + 8 * (n & 3)));
-      const uint2 av = __builtin_bit_cast(uint2, t4);
-      acc[bm] = M::pv(av, phi, acc[bm]);
-      acc[bm] = M::pv(av, plo, acc[bm]);
-    }
-  };
-
-  // Two tiles in flight: the next tile's loads are issued before the current
-  // tile is consumed, and no load is issued past the wave's last tile.
-  if (tok < end) {
-    for (;;) {
-      const int32_t tok1 = tok + tok_step, tok2 = tok1 + tok_step;
-      load(t[1], tok1);
-      step(t[0], tok, limit(t[0], tok));
-#if TC_DECODE_STAMPS
-      if (st_first == 0) st_first = __builtin_amdgcn_s_memrealtime();
-#endif
-      load(t[0], tok2);
-      if (tok1 < end) step(t[1], tok1, limit(t[1], tok1));
-      tok = tok2;
-      if (tok >= end) break;
-    }
-  }
-
-  if (APPEND && split == 0 && wave == 0) {
-    // The appended token as a tile whose only row is token 0 (the buffer
-    // range is one row, so the other rows read zero and are masked). Before
-    // the wave's own tiles it holds them up: 11.9 against 11.5 us at 10240
-    // tokens, 8.4 against 7.9 at 4000.
-    const char* kn = reinterpret_cast<const char*>(a.k_new + b * a.skn_b + h * a.skn_h);
-    const char* vn = reinterpret_cast<const char*>(a.v_new + b * a.svn_b + h * a.svn_h);
-    const __amdgpu_buffer_rsrc_t rk = make_rsrc(kn, kHeadDim * 2);
-    const __amdgpu_buffer_rsrc_t rv = make_rsrc(vn, kHeadDim * 2);
-    Tile tn;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      tn.k[j] = bload16(rk, 64 * j + 16 * g + n * kHeadDim * 2);
-      tn.v[j] = bload16(rv, (4 * g + j) * kHeadDim * 2 + 16 * n);
-    }
-    step(tn, 0, 1);
-    if (lane < 32) {
-      const bool is_v = lane >= 16;
-      const int chunk = 8 * (lane & 15);
-      const uint16_t* src = is_v ? a.v_new + b * a.svn_b + h * a.svn_h : a.k_new + b * a.skn_b + h * a.skn_h;
-      uint16_t* dst = nullptr;
-      if constexpr (PAGED) {
-        // The new token's slot: with device lengths, the offset table's row of
-        // position lens[b] (a position past the table's rows, or an offset
-        // outside the pool, writes nothing); otherwise the last row of the
-        // sequence's last tile (an invalid entry, or no tile, writes nothing).
-        if (plen >= 0) {
-          const int32_t off = plen < a.tok_pitch ? a.tok_off[static_cast<int64_t>(b) * a.tok_pitch + plen] : -1;
-          const int64_t room = static_cast<int64_t>(a.pages) * a.sk_b * 2 - h * a.sk_h * 2 - kHeadDim * 2;
-          if (off >= 0 && off <= room) {
-            char* base = reinterpret_cast<char*>(is_v ? a.v_w + h * a.sv_h : a.k_w + h * a.sk_h);
-            dst = reinterpret_cast<uint16_t*>(base + off);
-          }
-        } else if (last_tile >= 0) {
-          const int4 e = *reinterpret_cast<const int4*>(tab + 4 * last_tile);
-          if (!(e.x < 0 || e.x >= a.pages || e.y < 0 || e.z < 1 || e.z > 16 || e.y > a.page_tokens - e.z)) {
-            const int64_t slot = e.y + e.z - 1;
-            dst = is_v ? a.v_w + e.x * a.sv_b + h * a.sv_h + slot * a.sv_t
-                       : a.k_w + e.x * a.sk_b + h * a.sk_h + slot * a.sk_t;
-          }
-        }
-      } else {
-        dst = is_v ? a.v_w + b * a.sv_b + h * a.sv_h + last * a.sv_t : a.k_w + b * a.sk_b + h * a.sk_h + last * a.sk_t;
-      }
-      if (dst) *reinterpret_cast<uint4*>(dst + chunk) = *reinterpret_cast<const uint4*>(src + chunk);
-    }
-  }
-
-#if TC_DECODE_STAMPS
-  st_loop = __builtin_amdgcn_s_memrealtime();
-  auto record = [&]() {
-    if (a.stamps && lane == 0) {
-      unsigned long long* o =
-          a.stamps + (((static_cast<int64_t>(b) * a.heads + h) * a.splits + split) * W + wave) * 8;
-      o[0] = st_start; o[1] = st_first; o[2] = st_loop; o[3] = st_merge;
-      o[4] = __builtin_amdgcn_s_memrealtime();
-      o[5] = __builtin_amdgcn_s_getreg((31 << 11) | (0 << 6) | 4);   // HW_REG_HW_ID
-      o[6] = __builtin_amdgcn_s_getreg((15 << 11) | (0 << 6) | 20);  // HW_REG_XCC_ID
-    }
-  };
-#endif
-  // The head's sum over the four lane groups; m is already common to them.
-  l = rows_sum(l);
-  const int64_t part = (static_cast<int64_t>(b) * a.heads + h) * a.part_splits + a.part0 + split;
-  static_assert(W > 1, "the waves of a work-group are merged below");
-  if (n < a.group) {
-#pragma unroll
-    for (int bm = 0; bm < 8; ++bm)
-      *reinterpret_cast<float4*>(&s_acc[wave][n][16 * bm + 4 * g]) =
-          make_float4(acc[bm][0], acc[bm][1], acc[bm][2], acc[bm][3]);
-    if (g == 0) { s_m[n][wave] = m; s_l[n][wave] = l; }
-  }
-  // The split's output rows, addressed before the barrier (the address
-  // arithmetic is then off the path from the barrier to the stores).
-  float* const o_out = a.o_part + part * a.group * kHeadDim;
-  float* const l_out = a.lse_part + part * a.group;
-  __asm__ volatile("" ::"s"(o_out), "s"(l_out));
-  __syncthreads();
-#if TC_DECODE_STAMPS
-  st_merge = __builtin_amdgcn_s_memrealtime();
-#endif
-
-  // Each thread merges two adjacent dims of one head (one pass for G <= 4).
-  for (int idx = threadIdx.x; idx < a.group * (kHeadDim / 2); idx += 64 * W) {
-    const int hh = idx / (kHeadDim / 2);
-    const int d = 2 * (idx % (kHeadDim / 2));
-    float mw[W], lw[W];
-    float2 ow[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      mw[w] = s_m[hh][w];
-      lw[w] = s_l[hh][w];
-      ow[w] = *reinterpret_cast<const float2*>(&s_acc[w][hh][d]);
-    }
-    float Mx = neg_inf();
-#pragma unroll
-    for (int w = 0; w < W; ++w) Mx = fmaxf(Mx, mw[w]);
-    const float Ms = (Mx == neg_inf()) ? 0.f : Mx;
-    float L = 0.f, O0 = 0.f, O1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float f = __builtin_amdgcn_exp2f(mw[w] - Ms);
-      L += lw[w] * f;
-      O0 += ow[w].x * f;
-      O1 += ow[w].y * f;
-    }
-    // L >= 1 whenever a token was seen (the maximum contributes exp2(0)).
-    const float inv = L == 0.f ? 0.f : __builtin_amdgcn_rcpf(L);
-    float2 y = make_float2(O0 * inv, O1 * inv);
-    if constexpr (DIRECT) {
-      // Rounded to fp32 and then to the element type, as the combine reads and
-      // writes it (the compiler would take both steps in one v_fma_mix).
-      __asm__("" : "+v"(y.x), "+v"(y.y));
-      uint16_t* dst = a.out + b * a.so_b + h * a.so_h + hh * a.so_g + d;
-      *reinterpret_cast<uint32_t*>(dst) = E::bits(y.x) | (E::bits(y.y) << 16);
-      continue;
-    }
-    *reinterpret_cast<float2*>(o_out + hh * kHeadDim + d) = y;
-    if (d == 0) l_out[hh] = (L == 0.f) ? neg_inf() : (Mx + __builtin_amdgcn_logf(L)) * kLn2;
-  }
-#if TC_DECODE_STAMPS
-  record();
-#endif
+  decode_partial<DT, PAGED, APPEND, DIRECT, W, WINDOW>(a, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, threadIdx.x, s_vt,
+                                                       s_acc, s_m, s_l);
 }
 
 // x of the lane pair (l, l ^ 16) or (l, l ^ 32): the lower row's value in lo,
@@ -842,7 +424,8 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
                  int kv_heads, int group, int head_dim, int dtype, float scale, int split_tokens, int num_splits,
                  float* o_part_dev, float* lse_part_dev, int interleave, const Append* app, void* stream,
                  const Paged* paged = nullptr, bool whole_call = false, void* out_dev = nullptr,
-                 const int64_t* out_strides = nullptr, const Window* window = nullptr, int part0 = 0) {
+                 const int64_t* out_strides = nullptr, const Window* window = nullptr, int part0 = 0,
+                 PartialArgs* only = nullptr) {
   int rc = check_common(batch, kv_heads, group, head_dim, dtype);
   if (rc != TC_OK) return rc;
   if (n_tokens == 0 && num_splits == 0) return TC_OK;  // empty caches: nothing to read
@@ -923,6 +506,10 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
   a.stamps = g_stamps;
 #endif
 
+  if (only) {  // the caller launches
+    *only = a;
+    return TC_OK;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int waves = partial_waves(n_tokens, lens_dev != nullptr, paged != nullptr, app != nullptr, interleave,
                                   !whole_call || n_tokens <= int64_t(8) * kWaveIter * num_splits);
@@ -1314,18 +901,21 @@ struct Prefix {
   const int32_t* tiles = nullptr;
 };
 
-// Splits of a shared-prefix call: the prefix pass's come first.
+// Splits of a shared-prefix call: the prefix's come first.
 int shared_plan(int batch, int kv_heads, int group, int64_t prefix_tokens, int64_t max_tokens, int ragged, int* S_prefix,
                 int* S_own, int* T_own) {
   int cus = 0, rc;
-  if (batch < 1 || kv_heads < 1 || group < 1 || prefix_tokens < 0 || prefix_tokens > kMaxTokens)
-    return fail(TC_ERR_INVALID_ARGUMENT, "prefix of %lld tokens, batch %d, kv_heads %d, group %d",
-                (long long)prefix_tokens, batch, kv_heads, group);
-  if ((rc = split_plan(batch, kv_heads, max_tokens, 0, ragged, S_own, T_own)) != TC_OK) return rc;
-  *S_prefix = 0;
-  if (prefix_tokens == 0) return TC_OK;
+  if (batch < 1 || kv_heads < 1 || group < 1 || prefix_tokens < 0 || prefix_tokens > kMaxTokens || max_tokens < 0 ||
+      max_tokens > kMaxTokens)
+    return fail(TC_ERR_INVALID_ARGUMENT, "prefix of %lld and own %lld tokens, batch %d, kv_heads %d, group %d",
+                (long long)prefix_tokens, (long long)max_tokens, batch, kv_heads, group);
+  if (prefix_tokens == 0) {
+    *S_prefix = 0;
+    return split_plan(batch, kv_heads, max_tokens, 0, ragged, S_own, T_own);
+  }
   if ((rc = current_device_cus(&cus)) != TC_OK) return rc;
-  *S_prefix = prefix_splits(batch, kv_heads, group, ceil_div(prefix_tokens, kWaveIter), cus);
+  shared_splits(batch, kv_heads, group, ceil_div(prefix_tokens, kWaveIter), max_tokens, ragged != 0, cus, S_prefix, S_own);
+  *T_own = static_cast<int>(std::max<int64_t>(1, ceil_div(ceil_div(max_tokens, std::max(*S_own, 1)), kSplitGranule)) * kSplitGranule);
   return TC_OK;
 }
 
@@ -1361,10 +951,13 @@ int shared_impl(const void* q_dev, const int64_t q_strides[3], const Prefix& x, 
     return fail(TC_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed for %d splits", workspace_bytes, need, Sp + S);
   float* o_part = static_cast<float*>(workspace_dev);
   float* lse_part = o_part + static_cast<size_t>(batch) * kv_heads * (Sp + S) * group * head_dim;
-  // The own tokens first: their arguments are checked there, and nothing is enqueued if they are refused.
+  PartialArgs own{};
   if (S > 0 && (rc = partial_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch,
                                   kv_heads, group, head_dim, dtype, scale, t, S, o_part, lse_part, 1, app, stream,
-                                  paged, true, nullptr, nullptr, nullptr, Sp)) != TC_OK) return rc;
+                                  paged, true, nullptr, nullptr, nullptr, Sp, &own)) != TC_OK) return rc;
+#if TC_DECODE_STAMPS
+  own.stamps = nullptr;  // the timeline's buffer is laid out for the decode partial kernel's grid
+#endif
   PrefixArgs a;
   a.q = static_cast<const uint16_t*>(q_dev);
   a.k = static_cast<const uint16_t*>(x.k);
@@ -1391,7 +984,9 @@ int shared_impl(const void* q_dev, const int64_t q_strides[3], const Prefix& x, 
   // (A scale of 0 as one so small that every weight is 1: a hidden key's -inf times it stays -inf.)
   a.c = std::max(static_cast<float>(fabs(static_cast<double>(scale)) * 1.4426950408889634), 1e-30f);
   a.sign = scale < 0.f ? 0x80008000u : 0u;
-  if ((rc = hip_status(launch_prefix(a, dtype, static_cast<hipStream_t>(stream)), "prefix pass launch")) != TC_OK) return rc;
+  const int64_t shares = int64_t(Sp) * ceil_div(int64_t(batch) * group, 256) + int64_t(S) * batch;
+  if (shares * kv_heads > 0x7fffffff) return fail(TC_ERR_UNSUPPORTED, "grid too large");
+  if ((rc = hip_status(launch_shared(a, own, dtype, static_cast<hipStream_t>(stream)), "shared-prefix launch")) != TC_OK) return rc;
   return tc_decode_combine(o_part, lse_part, batch, kv_heads, group, head_dim, Sp + S, out_dev, out_strides, dtype,
                            stream);
 }

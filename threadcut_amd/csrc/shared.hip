@@ -4,10 +4,11 @@
 //   out_b = softmax([q_b Kp^T, q_b K_b^T] scale) [Vp; V_b]
 //
 // is the merge, by log-sum-exp, of the attention over the prefix and over each
-// sequence's own tokens. The second is the decode partial kernel; this file's
-// kernel is the first: for one KV head, the B*G query rows of all sequences
-// are the columns of the products that the decode kernel makes for the G rows
-// of one sequence, so a K/V tile in registers serves all of them.
+// sequence's own tokens. The second is the work of the decode partial kernel;
+// for the first, of one KV head, the B*G query rows of all sequences are the
+// columns of the products that the decode kernel makes for the G rows of one
+// sequence, so a K/V tile serves all of them. One launch does both: some
+// work-groups take shares of the prefix, the others sequences' own tokens.
 //
 // Per wave and step of 32 tokens (two 16-token tiles t = 0, 1), with column
 // n = lane % 16 of block r and lane group g = lane / 16:
@@ -53,22 +54,19 @@ struct Shape {
 // distinct banks.
 __device__ __forceinline__ int slot_of(int x, int r) { return x ^ (2 * ((r & 7) ^ (r >> 3 << 2)) + (r >> 3)); }
 
+// Split `split` of the prefix for head h and the columns of block `block`.
 template <int DT, bool PAGED, class S>
-__global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W / 4))) void prefix_partial_kernel(
-    const PrefixArgs a) {
+__device__ __forceinline__ void prefix_partial(const PrefixArgs& a, const int h, const int split, const int block,
+                                               char* const s_k0, char* const s_k1, char* const s_v0, char* const s_v1,
+                                               float (*s_m)[16], float (*s_l)[16]) {
   using M = DecodeMma<DT>;
   using E = Elem<DT>;
   constexpr int R = S::R, CG = S::CG, KG = S::KG;
-  __shared__ __attribute__((aligned(1024))) char s_k0[S::kBuf], s_k1[S::kBuf], s_v0[S::kBuf], s_v1[S::kBuf];
-  __shared__ float s_m[S::W][16], s_l[S::W][16];
-
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int cg = wave % CG, kg = wave / CG;
-  // Grid (heads, splits, column blocks), the KV head fastest: with 8 heads a head's work-groups share an XCD's L2.
-  const int h = blockIdx.x, split = blockIdx.y;
-  const int c0 = static_cast<int>(blockIdx.z) * S::kColumns + 16 * R * cg;
+  const int c0 = block * S::kColumns + 16 * R * cg;
   const int columns = a.batch * a.group;
   const char* kslab = reinterpret_cast<const char*>(a.k + h * a.sk_h);
   const char* vslab = reinterpret_cast<const char*>(a.v + h * a.sv_h);
@@ -347,6 +345,39 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
   }
 }
 
+// The grid: the KV head fastest (with 8 heads a head's work-groups share an
+// XCD's L2); then the prefix's splits and column blocks, then the sequences'
+// own tokens, which 4 waves take as in the decode partial kernel (so a
+// work-group of 8 takes two shares).
+template <int DT, bool PAGED, bool APPEND, class S>
+__global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W / 4))) void shared_partial_kernel(
+    const PrefixArgs a, const PartialArgs o) {
+  __shared__ __attribute__((aligned(1024))) char s_k0[S::kBuf], s_k1[S::kBuf], s_v0[S::kBuf], s_v1[S::kBuf];
+  __shared__ float s_m[S::W][16], s_l[S::W][16];
+  const uint32_t heads = a.heads, y = blockIdx.x / heads, h = blockIdx.x - y * heads;
+  const uint32_t shares = a.splits * static_cast<uint32_t>(a.blocks);
+  if (y < shares) {
+    const uint32_t block = y / a.splits;
+    prefix_partial<DT, PAGED, S>(a, h, y - block * a.splits, block, s_k0, s_k1, s_v0, s_v1, s_m, s_l);
+    return;
+  }
+  constexpr int kOwn = 4, kUnits = S::W / kOwn;
+  const int unit = kUnits > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * kOwn)) : 0;
+  const uint32_t j = (y - shares) * kUnits + unit, z = j / o.splits;
+  static_assert(kOwn * kVTileWords * 4 <= S::kBuf && kOwn * 8 * (kHeadDim + 16) * 4 <= S::kBuf, "a share's LDS");
+  char* const vt = unit ? s_v0 : s_k0;
+  char* const acc = unit ? s_v1 : s_k1;
+  static_assert(2 * 8 * kOwn <= S::W / kUnits * 16, "a share's maxima and sums");
+  float* const ml = unit ? s_l[0] : s_m[0];
+  if (z < static_cast<uint32_t>(a.batch))
+    decode_partial<DT, PAGED, APPEND, false, kOwn, false>(
+        o, h, j - z * o.splits, z, a.batch, threadIdx.x - unit * 64 * kOwn, reinterpret_cast<uint32_t(*)[kVTileWords]>(vt),
+        reinterpret_cast<float(*)[8][kHeadDim + 16]>(acc), reinterpret_cast<float(*)[kOwn]>(ml),
+        reinterpret_cast<float(*)[kOwn]>(ml + 8 * kOwn));
+  else
+    __syncthreads();  // the one that the other half of the work-group meets in its merge
+}
+
 // The shape of a call: all columns in one work-group up to 256, else in blocks of them.
 struct Plan {
   int cg, r;
@@ -361,42 +392,59 @@ Plan shape_plan(int batch, int group) {
   return Plan{cg, 2, ceil_div(c, 256)};
 }
 
-template <int DT, bool PAGED, int W, int CG, int R>
-void launch_shape(const PrefixArgs& a, int64_t blocks, hipStream_t s) {
-  using S = Shape<W, CG, R>;
-  hipLaunchKernelGGL((prefix_partial_kernel<DT, PAGED, S>), dim3(a.heads, a.splits, static_cast<unsigned>(blocks)),
-                     dim3(64 * W), 0, s, a);
+template <int DT, bool PAGED, bool APPEND, int W, int CG, int R>
+void launch_shape(const PrefixArgs& a, const PartialArgs& o, hipStream_t s) {
+  constexpr int kUnits = W / 4;
+  const int64_t rows = static_cast<int64_t>(a.splits) * a.blocks + ceil_div(static_cast<int64_t>(o.splits) * a.batch, kUnits);
+  hipLaunchKernelGGL((shared_partial_kernel<DT, PAGED, APPEND, Shape<W, CG, R>>), dim3(static_cast<unsigned>(a.heads * rows)),
+                     dim3(64 * W), 0, s, a, o);
 }
 
-template <int DT, bool PAGED>
-void launch(const PrefixArgs& a, hipStream_t s) {
-  const Plan p = shape_plan(a.batch, a.group);
+template <int DT, bool PAGED, bool APPEND>
+void launch(const PrefixArgs& a, const PartialArgs& o, const Plan& p, hipStream_t s) {
   switch (p.cg) {
     case 1:
-      if (p.r == 1) return launch_shape<DT, PAGED, 4, 1, 1>(a, p.blocks, s);
-      return launch_shape<DT, PAGED, 4, 1, 2>(a, p.blocks, s);
-    case 2: return launch_shape<DT, PAGED, 8, 2, 2>(a, p.blocks, s);
-    case 4: return launch_shape<DT, PAGED, 8, 4, 2>(a, p.blocks, s);
-    default: return launch_shape<DT, PAGED, 8, 8, 2>(a, p.blocks, s);
+      if (p.r == 1) return launch_shape<DT, PAGED, APPEND, 4, 1, 1>(a, o, s);
+      return launch_shape<DT, PAGED, APPEND, 4, 1, 2>(a, o, s);
+    case 2: return launch_shape<DT, PAGED, APPEND, 8, 2, 2>(a, o, s);
+    case 4: return launch_shape<DT, PAGED, APPEND, 8, 4, 2>(a, o, s);
+    default: return launch_shape<DT, PAGED, APPEND, 8, 8, 2>(a, o, s);
   }
+}
+
+template <int DT>
+void launch_dt(const PrefixArgs& a, const PartialArgs& o, const Plan& p, hipStream_t s) {
+  if (!a.tile_tab) return launch<DT, false, false>(a, o, p, s);
+  if (o.k_new) return launch<DT, true, true>(a, o, p, s);
+  launch<DT, true, false>(a, o, p, s);
 }
 
 }  // namespace
 
-// As many work-groups as compute units (one fits a unit), but a group of tiles for every one.
-int prefix_splits(int batch, int heads, int group, int64_t tiles, int cus) {
+// One work-group fits a compute unit, so the units are dealt to the prefix and to the own tokens by what each has to
+// read, and each share is cut into as many splits as it has units.
+void shared_splits(int batch, int heads, int group, int64_t prefix_tiles, int64_t own_tokens, bool ragged, int cus,
+                   int* prefix, int* own) {
   const Plan p = shape_plan(batch, group);
-  const int64_t per_split = heads * p.blocks;
-  const int64_t most = ceil_div(tiles, 8);
-  return static_cast<int>(std::max<int64_t>(tiles > 0, std::min<int64_t>({cus / per_split, most, 1024})));
+  const int64_t per_split = heads * p.blocks, most = ceil_div(prefix_tiles, 8), tiles = ceil_div(own_tokens, kWaveIter);
+  const double wp = 16.0 * prefix_tiles * heads * p.blocks * (p.cg == 8 ? 1.5 : 1.0);
+  const double wo = own_tokens * static_cast<double>(batch) * heads * (ragged ? 0.6 : 1.0);
+  const int64_t mine = static_cast<int64_t>(cus * wp / (wp + wo) + 0.5);
+  const int64_t sp = std::max<int64_t>(1, std::min<int64_t>({mine / per_split, most, 1024}));
+  const int64_t left = std::max<int64_t>(cus - sp * per_split, cus / 8) * (p.cg == 1 ? 1 : 2) * (ragged ? 2 : 1);
+  const int64_t pairs = static_cast<int64_t>(batch) * heads;
+  *prefix = static_cast<int>(sp);
+  *own = static_cast<int>(tiles ? std::max<int64_t>(1, std::min<int64_t>({(left + pairs / 2) / pairs, ceil_div(tiles, 4), 1024})) : 0);
 }
 
-hipError_t launch_prefix(const PrefixArgs& a, int dtype, hipStream_t stream) {
-  if (dtype == TC_DTYPE_F16) {
-    if (a.tile_tab) launch<TC_DTYPE_F16, true>(a, stream); else launch<TC_DTYPE_F16, false>(a, stream);
-  } else {
-    if (a.tile_tab) launch<TC_DTYPE_BF16, true>(a, stream); else launch<TC_DTYPE_BF16, false>(a, stream);
-  }
+hipError_t launch_shared(const PrefixArgs& a_in, const PartialArgs& o, int dtype, hipStream_t stream) {
+  PrefixArgs a = a_in;
+  const Plan p = shape_plan(a.batch, a.group);
+  a.blocks = static_cast<int>(p.blocks);
+  if (dtype == TC_DTYPE_F16)
+    launch_dt<TC_DTYPE_F16>(a, o, p, stream);
+  else
+    launch_dt<TC_DTYPE_BF16>(a, o, p, stream);
   return hipGetLastError();
 }
 

@@ -1,10 +1,12 @@
-// The prefix pass of shared-prefix decode (shared.hip), which decode.hip's
-// entry points launch beside the partial kernel of each sequence's own tokens.
+// The partial pass of shared-prefix decode (shared.hip): the prefix for all
+// sequences, and each sequence's own tokens, in one launch.
 #pragma once
 
 #include "tc_common.hpp"
 
 namespace tc {
+
+struct PartialArgs;  // decode_tile.hpp
 
 struct PrefixArgs {
   const uint16_t* q;        // [B, H, G, D]
@@ -21,12 +23,17 @@ struct PrefixArgs {
   int32_t pages, page_tokens;
   int heads, group, batch;
   int splits, part_splits;
+  int blocks;               // blocks of columns (set by launch_shared)
   float c;                  // |scale| log2(e), > 0
   uint32_t sign;            // 0x80008000 for a negative scale: flips the queries
 };
 
-// Splits of the prefix pass for `tiles` tiles, and the launch itself.
-int prefix_splits(int batch, int heads, int group, int64_t tiles, int cus);
-hipError_t launch_prefix(const PrefixArgs& a, int dtype, hipStream_t stream);
+// Splits of the prefix (a.splits) and of the sequences' own tokens for a call on `cus` compute units: prefix tiles of 16
+// tokens, own_tokens of the longest sequence.
+void shared_splits(int batch, int heads, int group, int64_t prefix_tiles, int64_t own_tokens, bool ragged, int cus,
+                   int* prefix, int* own);
+
+// The launch: a for the prefix; o (its splits from a.splits on) for the own tokens, whose splits may be 0.
+hipError_t launch_shared(const PrefixArgs& a, const PartialArgs& o, int dtype, hipStream_t stream);
 
 }  // namespace tc
