@@ -190,6 +190,12 @@ class Forked:
             close(out[i], *definition(q[i], r[0, layer], r[1, layer]), q.shape[0] * q.shape[2])
 
 
+def few(monkeypatch):
+    """Short prefixes are read once too (by default they take the plain call, which is faster there)."""
+    monkeypatch.setattr(paged, "SHARED_MIN_ROWS", 2048)
+    monkeypatch.setattr(paged, "SHARED_MIN_ROWS_FEW", 2048)
+
+
 @pytest.fixture(params=["native", "Python"])
 def calls(request, monkeypatch):
     """Which decode calls read the prefix once, through either path of the wrappers."""
@@ -206,6 +212,7 @@ def calls(request, monkeypatch):
 
     fast.paged_shared = native
     monkeypatch.setattr(_lib, "FAST", fast if request.param == "native" else None)
+    few(monkeypatch)
     monkeypatch.setattr(paged.PagedKV, "_attend_shared", lambda self, *a: taken.append(2) or attend(self, *a))
     yield taken
     assert set(taken) == {1 if request.param == "native" else 2}
@@ -274,9 +281,12 @@ def test_what_is_shared_changes(gpu, calls):
         f.cache.fork(0, 2)
 
 
-def test_the_paged_operators_together(gpu):
+@pytest.mark.parametrize("short", [True, False])
+def test_the_paged_operators_together(gpu, monkeypatch, short):
     """A prompt, forks of it, a chunk of new tokens and decode steps, keys and queries rotated on the way, with and
     without a window: against float64 from the rows as they were handed over."""
+    if short:
+        few(monkeypatch)
     b, heads, g, prefix, chunk = 3, 8, 4, 700, 40
     inv = workloads.inv_freq().to(gpu)
     cache = paged.PagedKV(2, heads, 60, 64, batch=b, device=gpu)
@@ -325,7 +335,8 @@ def test_the_paged_operators_together(gpu):
         n += t
 
 
-def test_fork_on_another_stream(gpu):
+def test_fork_on_another_stream(gpu, monkeypatch):
+    few(monkeypatch)
     f = Forked(gpu, 600, [10, 20], 64)
     q = rand(1, (2, 8, 4, D), torch.float16, gpu)
     first = f.cache.decode(0, q, SCALE)
@@ -358,3 +369,17 @@ def test_bad_tiles_count_as_empty(gpu):
     v = torch.cat((vpool[0, :, :16], vpool[3, :, 16:], vpool[2, :, 31:]), 1)
     for i in range(3):
         close(out[i], *definition(q[i], k, v), 12)
+
+
+def test_what_pays(gpu):
+    """By default short prefixes, and few sequences, take the plain call."""
+    x = torch.zeros(8, 2100, D, dtype=torch.float16, device=gpu)
+    for b, prefix, group, pays in ((2, 2100, 4, False), (4, 2100, 4, True), (4, 1000, 4, False), (4, 2100, 8, False),
+                                   (8, 2100, 4, False), (9, 2100, 4, True), (8, 900, 2, True), (17, 1100, 4, True),
+                                   (3, 2100, 16, False)):
+        c = paged.PagedKV(1, 8, 34, 64, batch=b, device=gpu)
+        c.append(0, [x[:, :prefix]], [x[:, :prefix]])
+        assert c.shared_tables(group) is None
+        for i in range(1, b):
+            c.fork(0, i)
+        assert (c.shared_tables(group) is not None) == pays, (b, prefix, group)

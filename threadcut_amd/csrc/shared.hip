@@ -422,16 +422,19 @@ void launch_dt(const PrefixArgs& a, const PartialArgs& o, const Plan& p, hipStre
 }  // namespace
 
 // One work-group fits a compute unit, so the units are dealt to the prefix and to the own tokens by what each has to
-// read, and each share is cut into as many splits as it has units.
+// read, and each share is cut into as many splits as it has units. Eight column groups make the prefix bound by its
+// products: a tile weighs twice there (64 x 16384 tokens of 4 rows: 84 us; weights of 1.5, 2.5 and 3 were 2 to 6 us
+// slower). Ragged own tokens weigh less, as their longest is given here. Twice the splits for them cost 24 forked
+// sequences 3 %: more partials to join than the longest sequence loses.
 void shared_splits(int batch, int heads, int group, int64_t prefix_tiles, int64_t own_tokens, bool ragged, int cus,
                    int* prefix, int* own) {
   const Plan p = shape_plan(batch, group);
   const int64_t per_split = heads * p.blocks, most = ceil_div(prefix_tiles, 8), tiles = ceil_div(own_tokens, kWaveIter);
-  const double wp = 16.0 * prefix_tiles * heads * p.blocks * (p.cg == 8 ? 1.5 : 1.0);
+  const double wp = 16.0 * prefix_tiles * heads * p.blocks * (p.cg == 8 ? 2.0 : 1.0);
   const double wo = own_tokens * static_cast<double>(batch) * heads * (ragged ? 0.6 : 1.0);
   const int64_t mine = static_cast<int64_t>(cus * wp / (wp + wo) + 0.5);
   const int64_t sp = std::max<int64_t>(1, std::min<int64_t>({mine / per_split, most, 1024}));
-  const int64_t left = std::max<int64_t>(cus - sp * per_split, cus / 8) * (p.cg == 1 ? 1 : 2) * (ragged ? 2 : 1);
+  const int64_t left = std::max<int64_t>(cus - sp * per_split, cus / 8) * (p.cg == 1 ? 1 : 2);
   const int64_t pairs = static_cast<int64_t>(batch) * heads;
   *prefix = static_cast<int>(sp);
   *own = static_cast<int>(tiles ? std::max<int64_t>(1, std::min<int64_t>({(left + pairs / 2) / pairs, ceil_div(tiles, 4), 1024})) : 0);

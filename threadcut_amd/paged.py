@@ -42,7 +42,15 @@ from .kv import _plain, rope_table, rotate_half, rows_ok, watched
 from .prefill import GROUPS, band_mask
 
 TILE = 16  # rows per tile-table entry (the decode kernel's tile)
-SHARED_MIN_TOKENS = 256  # tokens that all sequences share, from which decode reads them once for all
+# Rows of K (tokens times KV heads) whose repeated reading has to be saved for decode to read what all sequences share
+# once for all: the one launch for both, with large work-groups, takes longer than the plain one where there is little
+# to save. At most 16 query rows a KV head (of more than two sequences) take a lighter work-group. Shared against plain
+# (us on the GPU, sequences of 60 to 200 own tokens, 8 KV heads, sequences x rows of a head): 4 x 4 1024 shared tokens
+# 8.1, 7.4, 2048 8.2, 8.6; 8 x 2 1024 8.2, 8.7; 2 x 4 8192 13.4, 11.8; 8 x 4 1024 10.5, 8.8, 2048 10.6, 11.4;
+# 16 x 4 512 12.4, 9.7, 1024 12.6, 13.0; 16 x 8 1024 14.4, 14.5; 32 x 4 512 15.9, 14.4, 1024 15.8, 22.0; of 2 KV
+# heads: 8 x 4 8192 12.1, 11.7; 16 x 4 4096 13.2, 12.0, 8192 14.5, 17.9.
+SHARED_MIN_ROWS = 131072
+SHARED_MIN_ROWS_FEW = 49152
 _I64P = ctypes.POINTER(ctypes.c_int64)
 
 
@@ -513,21 +521,25 @@ class PagedKV:
         return (copies.get(_lib.raw_stream(self.device.index))
                 or _lib.per_stream(copies, self.device.index, self._upload_table))
 
-    def shared_tables(self):
+    def shared_tables(self, group):
         """(the tiles that every sequence begins with, int32 [T, 4], each sequence's own in device_table's form, on
-        the device) of a cache with forked sequences, or None where they share less than pays."""
+        the device) of a cache with forked sequences, or None where they share less than pays (for `group` query
+        heads a KV head)."""
         if not self.table.users:
             return None
         version, copies = self._dev_shared
         if version != self.table.version:
             t, head = self.table.shared_frags(), self.table.frags[0]
             copies = False
-            if t and int(head[:t, 2].sum()) >= SHARED_MIN_TOKENS:
-                copies = (_tiles(head[:t], self.table.page_tokens), *self.table.tile_table(skip=t), {})
+            if t:
+                saved = (self.table.batch - 1) * int(head[:t, 2].sum()) * self.kv_heads
+                copies = (saved, _tiles(head[:t], self.table.page_tokens), *self.table.tile_table(skip=t), {})
             self._dev_shared = (self.table.version, copies)
         if copies is False:
             return None
-        head, own, cnt, streams = copies
+        saved, head, own, cnt, streams = copies
+        if saved < (SHARED_MIN_ROWS_FEW if 2 < self.table.batch <= 16 // group else SHARED_MIN_ROWS):
+            return None
         return (streams.get(_lib.raw_stream(self.device.index))
                 or _lib.per_stream(streams, self.device.index, lambda: _upload((head, own, cnt), self.device)))
 
@@ -688,12 +700,12 @@ class PagedKV:
         """
         self._refuse_during_step("decode", layer)
         fast = _lib.FAST
-        if fast is not None and split is None and q.is_cuda and 0 <= layer < self.layers:
+        if fast is not None and split is None and q.is_cuda and q.dim() == 4 and 0 <= layer < self.layers:
             # The whole call in native code; None for what it does not take (then as below).
             stream = _lib.raw_stream(self.device.index)
-            key = (self.table.version, window, sink_tokens, stream)
+            key = (self.table.version, window, sink_tokens, stream, q.shape[2])
             if self._last_tables[0] != key:  # the layers of a step ask for the same ones
-                shared = self.shared_tables() if window is None else None
+                shared = self.shared_tables(q.shape[2]) if window is None else None
                 self._last_tables = (key, shared, None if shared else self.window_table(window, sink_tokens, "decode"))
             _, shared, table = self._last_tables
             if shared:
@@ -718,7 +730,7 @@ class PagedKV:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
             raise ValueError("PagedKV.decode: out must match q in shape, dtype and device")
-        tables = self.shared_tables() if window is None and split is None else None
+        tables = self.shared_tables(g) if window is None and split is None else None
         if tables is not None:
             return self._attend_shared(tables, layer, q, None, None, scale, out)
         tab, cnt, mt = self.window_table(window, sink_tokens, "decode")
@@ -819,10 +831,10 @@ class PagedKV:
         step, fast = getattr(self, "_step", None), _lib.FAST
         if step is not None and step[2] != 1 and step[0] == self.table.version:
             raise RuntimeError(f"PagedKV.decode_append: the step has {step[2]} tokens a sequence (write_step takes them)")
-        if (fast is not None and split is None and q.is_cuda and step is not None and step[0] == self.table.version
-                and layer in step[1]):
+        if (fast is not None and split is None and q.is_cuda and q.dim() == 4 and step is not None
+                and step[0] == self.table.version and layer in step[1]):
             # The whole call in native code; None for what it does not take (then as below).
-            tables = self.shared_tables() if window is None else None
+            tables = self.shared_tables(q.shape[2]) if window is None else None
             stream = _lib.raw_stream(q.get_device())
             if tables is not None:
                 done = fast.paged_shared(q, self.k_pools[layer], self.v_pools[layer], *tables, k_new, v_new, out, scale,
@@ -855,7 +867,7 @@ class PagedKV:
             out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
             raise ValueError("PagedKV.decode_append: out must match q in shape, dtype and device")
-        tables = self.shared_tables() if window is None and split is None else None
+        tables = self.shared_tables(g) if window is None and split is None else None
         if tables is not None:
             self._attend_shared(tables, layer, q, kn, vn, scale, out)
             step[1].discard(layer)
