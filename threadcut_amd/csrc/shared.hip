@@ -423,9 +423,11 @@ void launch_dt(const PrefixArgs& a, const PartialArgs& o, const Plan& p, hipStre
 
 // One work-group fits a compute unit, so the units are dealt to the prefix and to the own tokens by what each has to
 // read, and each share is cut into as many splits as it has units. Eight column groups make the prefix bound by its
-// products: a tile weighs twice there (64 x 16384 tokens of 4 rows: 84 us; weights of 1.5, 2.5 and 3 were 2 to 6 us
-// slower). Ragged own tokens weigh less, as their longest is given here. Twice the splits for them cost 24 forked
-// sequences 3 %: more partials to join than the longest sequence loses.
+// products, so a tile weighs twice there: 64 sequences x 4 rows over 16384 tokens take 85.5 us, with a weight of 1,
+// 1.5 and 3 118.8, 95.7 and 94.6. Ragged own tokens, whose longest is given here, weigh 0.6: with 1 those took 105.6
+// us, 32 x 4 rows over 8000 tokens 46.9 instead of 34.8 (40 x 2 over 3000 16.6 instead of 18.5). Twice the splits for
+// ragged own tokens helped the longest sequence of some batches (60 x 8 rows: 50.2 us instead of 58.9; 24 forked ones
+// 335 instead of 343) and cost others more than that in joining (12 x 8 forked: 77.9 instead of 64.3; 5 x 4 73 from 63).
 void shared_splits(int batch, int heads, int group, int64_t prefix_tiles, int64_t own_tokens, bool ragged, int cus,
                    int* prefix, int* own) {
   const Plan p = shape_plan(batch, group);
