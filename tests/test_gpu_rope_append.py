@@ -283,3 +283,23 @@ def test_rows_that_do_not_fit_change_nothing(gpu):
             cache.append(0, ks, vs, inv_freq=inv)
     assert (cache.table.frags[0] == table).all() and cache.table.free == free
     assert all(torch.equal(a, b) for a, b in zip(cache.k_pools + cache.v_pools, pools))
+
+
+def test_a_refused_append_takes_no_slots(gpu):
+    """Rows on the host, or a call inside a capture: the sequence and the free pages stay as they were."""
+    inv = workloads.inv_freq().to(gpu)
+    cache = paged.PagedKV(1, 2, 9, 16, device=gpu)
+    x = rand(1, (1, 2, 20, D), torch.float16, gpu)
+    cache.append(0, [x], [x], inv_freq=inv)
+    table, free = cache.table.frags[0].copy(), list(cache.table.free)
+    with pytest.raises(RuntimeError):
+        cache.append(0, [x.cpu()], [x.cpu()], inv_freq=inv)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        with pytest.raises(RuntimeError, match="not captured"):
+            cache.append(0, [x], [x], inv_freq=inv)
+    assert (cache.table.frags[0] == table).all() and cache.table.free == free and y is not None
+    cache.append(0, [x], [x], inv_freq=inv)
+    close(cache.gather(0)[0][:, 20:], x[0], 20, inv)

@@ -383,3 +383,40 @@ def test_what_pays(gpu):
         for i in range(1, b):
             c.fork(0, i)
         assert (c.shared_tables(group) is not None) == pays, (b, prefix, group)
+
+
+@pytest.mark.parametrize("window", [None, 300])
+def test_paged_calls_captured_and_replayed(gpu, monkeypatch, window):
+    """Forked and windowed decode of pages in a graph, after an eager call (which uploads the tables): every replay
+    against the eager call on the same queries, with eager calls between them."""
+    few(monkeypatch)
+    b, heads, g = 4, 8, 4
+    c = paged.PagedKV(1, heads, 60, 64, batch=b, device=gpu)
+    x = rand(1, (heads, 900, D), torch.float16, gpu)
+    c.append(0, [x], [x])
+    for i in range(1, b):
+        c.fork(0, i)
+        c.append(i, [x[:, :30 * i]], [x[:, 5:5 + 30 * i]])
+    q = rand(2, (b, heads, g, D), torch.float16, gpu)
+    c.decode(0, q, SCALE, window=window)
+    assert (c.shared_tables(g) is not None)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = c.decode(0, q, SCALE, window=window)
+    for seed in range(3, 7):
+        q.copy_(rand(seed, q.shape, q.dtype, gpu))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, c.decode(0, q, SCALE, window=window))
+
+
+def test_no_query_heads(gpu, monkeypatch):
+    few(monkeypatch)
+    c = paged.PagedKV(1, 8, 40, 64, batch=3, device=gpu)
+    x = torch.zeros(8, 600, D, dtype=torch.float16, device=gpu)
+    c.append(0, [x], [x])
+    for i in (1, 2):
+        c.fork(0, i)
+    with pytest.raises((ValueError, RuntimeError)):
+        c.decode(0, x.new_empty(3, 8, 0, D), SCALE)

@@ -314,7 +314,9 @@ def test_paged_cache_behind_the_attention(gpu, group):
 
 @pytest.mark.parametrize("form", ["float32", "host", "group 16"])
 def test_calls_the_kernels_do_not_take(gpu, form):
-    """They keep torch's attention, with the band as its mask."""
+    """They keep torch's attention, with the band as its mask. With u half a step of the type and S the largest sum of
+    |q k| scale: both factors and the score may be rounded to the type, and 128 terms added in fp32, so a score is off by
+    (3 u + 128 2^-24) S, a weight by twice that (itself and the sum of weights) and 2 u, and the result by u again."""
     dev, dtype, hq = (gpu, torch.float16, 16 * 2) if form == "group 16" else (torch.device("cpu") if form == "host" else gpu,
                                                                              torch.float32, 8)
     for t in (1, 30):
@@ -322,7 +324,10 @@ def test_calls_the_kernels_do_not_take(gpu, form):
         q = rand(3, (1, hq, t, D), dtype, dev)
         out = attention.attention(None, q, k, v, None, scaling=SCALE, sliding_window=40, sink_tokens=3)[0]
         want, spread = definition(q[0], k[0], v[0], 200 - t, 40, 3)
-        assert (out[0].transpose(0, 1).double() - want).abs().max() <= (2e-3 if dtype == torch.float16 else 1e-5)
+        u = torch.finfo(dtype).eps / 2
+        most = SCALE * max((q[0].double().abs() @ h.double().abs().t().contiguous()).max().item() for h in k[0])
+        bound = spread * (2 * (3 * u + 128 * 2.0 ** -24) * most + 2 * u) + u * want.abs()
+        assert torch.all((out[0].transpose(0, 1).double() - want).abs() <= bound)
 
 
 def test_extreme_scores(gpu):

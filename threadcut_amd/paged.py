@@ -403,25 +403,27 @@ class PagedKV:
             self._check_rows(ks, vs, n)
         if inv_freq is not None:
             _check_inv_freq(inv_freq, "append")
+            if torch.cuda.is_current_stream_capturing():  # (a replay would write the same slots again)
+                raise RuntimeError("PagedKV.append: rotated rows are not captured")
         start = self.table.length(b)
         slots = self.table.reserve(b, n)
         if n == 0:
             return
         if inv_freq is not None and self.layers:
-            at = _to_device(_placed(slots, start)[None], self.device)
-            if native:
-                if _lib.FAST.rope_rows(ks, vs, self.k_pools, self.v_pools, at, inv_freq, None,
-                                       _lib.raw_stream(self.device.index)):
-                    return
-                try:
+            try:
+                at = _to_device(_placed(slots, start)[None], self.device)
+                if native:
+                    if _lib.FAST.rope_rows(ks, vs, self.k_pools, self.v_pools, at, inv_freq, None,
+                                           _lib.raw_stream(self.device.index)):
+                        return
                     self._check_rows(ks, vs, n)
-                except ValueError:
-                    self.table.prune(b, start, start + n, 0)
-                    raise
-            ks, vs = [_as_batch(t) for t in ks], [_as_batch(t) for t in vs]
-            if self._write_rotated(range(self.layers), ks, vs, at, inv_freq):
-                return
-            ks = [_rotated(t.reshape(1, self.kv_heads, n, HEAD_DIM), at[..., 2], inv_freq) for t in ks]
+                ks, vs = [_as_batch(t) for t in ks], [_as_batch(t) for t in vs]
+                if self._write_rotated(range(self.layers), ks, vs, at, inv_freq):
+                    return
+                ks = [_rotated(t.reshape(1, self.kv_heads, n, HEAD_DIM), at[..., 2], inv_freq) for t in ks]
+            except Exception:
+                self.table.prune(b, start, start + n, 0)  # the sequence is as it was
+                raise
         idx = _to_device(slots, self.device)
         if self.layers and self._write_rows(range(self.layers), [_as_batch(t) for t in ks], [_as_batch(t) for t in vs],
                                             idx):
@@ -538,7 +540,7 @@ class PagedKV:
         if copies is False:
             return None
         saved, head, own, cnt, streams = copies
-        if saved < (SHARED_MIN_ROWS_FEW if 2 < self.table.batch <= 16 // group else SHARED_MIN_ROWS):
+        if saved < (SHARED_MIN_ROWS_FEW if self.table.batch > 2 and self.table.batch * group <= 16 else SHARED_MIN_ROWS):
             return None
         return (streams.get(_lib.raw_stream(self.device.index))
                 or _lib.per_stream(streams, self.device.index, lambda: _upload((head, own, cnt), self.device)))
