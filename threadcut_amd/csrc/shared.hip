@@ -425,19 +425,26 @@ void launch_dt(const PrefixArgs& a, const PartialArgs& o, const Plan& p, hipStre
 // read, and each share is cut into as many splits as it has units. Eight column groups make the prefix bound by its
 // products, so a tile weighs twice there: 64 sequences x 4 rows over 16384 tokens take 85.5 us, with a weight of 1,
 // 1.5 and 3 118.8, 95.7 and 94.6. Ragged own tokens, whose longest is given here, weigh 0.6: with 1 those took 105.6
-// us, 32 x 4 rows over 8000 tokens 46.9 instead of 34.8 (40 x 2 over 3000 16.6 instead of 18.5). Twice the splits for
-// ragged own tokens helped the longest sequence of some batches (60 x 8 rows: 50.2 us instead of 58.9; 24 forked ones
-// 335 instead of 343) and cost others more than that in joining (12 x 8 forked: 77.9 instead of 64.3; 5 x 4 73 from 63).
+// us, 32 x 4 rows over 8000 tokens 46.9 instead of 34.8. A sequence's own share costs as much as 64 tokens before its
+// first, and where there are few sequences they find units of their own; every split gets the same number of tile
+// groups, as the longest one counts (both: 40 x 2 rows over 3000 tokens with 60 own 15.0 us instead of 18.5, 20 x 8
+// over 12000 with 20 own 29.3 instead of 32.7, 2 x 4 over 16000 17.5 instead of 19.9, 24 x 4 forked 27.1 a layer
+// instead of 28.3; nothing slower). Twice the splits for ragged own tokens helped the longest sequence of some batches
+// (60 x 8 rows over 500: 50.2 us instead of 58.9) and cost others more in joining (12 x 8 forked: 19.5 instead of 16.1).
 void shared_splits(int batch, int heads, int group, int64_t prefix_tiles, int64_t own_tokens, bool ragged, int cus,
                    int* prefix, int* own) {
   const Plan p = shape_plan(batch, group);
   const int64_t per_split = heads * p.blocks, most = ceil_div(prefix_tiles, 8), tiles = ceil_div(own_tokens, kWaveIter);
   const double wp = 16.0 * prefix_tiles * heads * p.blocks * (p.cg == 8 ? 2.0 : 1.0);
-  const double wo = own_tokens * static_cast<double>(batch) * heads * (ragged ? 0.6 : 1.0);
-  const int64_t mine = static_cast<int64_t>(cus * wp / (wp + wo) + 0.5);
-  const int64_t sp = std::max<int64_t>(1, std::min<int64_t>({mine / per_split, most, 1024}));
-  const int64_t left = std::max<int64_t>(cus - sp * per_split, cus / 8) * (p.cg == 1 ? 1 : 2);
   const int64_t pairs = static_cast<int64_t>(batch) * heads;
+  const double wo = pairs * (own_tokens * (ragged ? 0.6 : 1.0) + 64);
+  const int64_t cap = cus - std::min<int64_t>(pairs, cus / 8);
+  const int64_t mine = std::min(static_cast<int64_t>(cus * wp / (wp + wo)), cap);
+  int64_t sp = std::max<int64_t>(1, std::min<int64_t>({(mine + per_split / 2) / per_split, most, 1024}));
+  int64_t each = (2 * most + sp) / (2 * sp);  // groups of a split
+  if (ceil_div(most, each) * per_split > std::max(cap, sp * per_split)) ++each;
+  sp = ceil_div(most, each);
+  const int64_t left = std::max<int64_t>(cus - sp * per_split, cus / 8) * (p.cg == 1 ? 1 : 2);
   *prefix = static_cast<int>(sp);
   *own = static_cast<int>(tiles ? std::max<int64_t>(1, std::min<int64_t>({(left + pairs / 2) / pairs, ceil_div(tiles, 4), 1024})) : 0);
 }

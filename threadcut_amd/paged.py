@@ -44,11 +44,11 @@ from .prefill import GROUPS, band_mask
 TILE = 16  # rows per tile-table entry (the decode kernel's tile)
 # Rows of K (tokens times KV heads) whose repeated reading has to be saved for decode to read what all sequences share
 # once for all: the one launch for both, with large work-groups, takes longer than the plain one where there is little
-# to save. At most 16 query rows a KV head (of more than two sequences) take a lighter work-group. Shared against plain
-# (us on the GPU, sequences of 60 to 200 own tokens, 8 KV heads, sequences x rows of a head): 4 x 4 1024 shared tokens
-# 8.1, 7.4, 2048 8.2, 8.6; 8 x 2 1024 8.2, 8.7; 2 x 4 8192 13.4, 11.8; 8 x 4 1024 10.5, 8.8, 2048 10.6, 11.4;
-# 16 x 4 512 12.4, 9.7, 1024 12.6, 13.0; 16 x 8 1024 14.4, 14.5; 32 x 4 512 15.9, 14.4, 1024 15.8, 22.0; of 2 KV
-# heads: 8 x 4 8192 12.1, 11.7; 16 x 4 4096 13.2, 12.0, 8192 14.5, 17.9.
+# to save. At most 16 query rows a KV head take a lighter work-group. Shared against plain (us on the GPU, sequences of
+# 60 to 200 own tokens, 8 KV heads, sequences x rows of a head): 2 x 4 4096 shared tokens 8.9, 8.5, 8192 10.8, 11.8;
+# 4 x 4 1024 8.1, 7.4, 2048 8.1, 8.7; 8 x 2 1024 8.2, 8.8; 8 x 4 1024 10.5, 9.0, 2048 10.7, 11.5; 16 x 4 512 12.5,
+# 9.8, 1024 12.7, 13.0; 16 x 8 1024 14.4, 14.6; 32 x 4 512 14.2, 14.4, 1024 16.1, 21.9; of 2 KV heads: 8 x 4 8192
+# 12.1, 11.9; 16 x 4 4096 13.1, 12.3, 8192 14.7, 18.3.
 SHARED_MIN_ROWS = 131072
 SHARED_MIN_ROWS_FEW = 49152
 _I64P = ctypes.POINTER(ctypes.c_int64)
@@ -540,7 +540,7 @@ class PagedKV:
         if copies is False:
             return None
         saved, head, own, cnt, streams = copies
-        if saved < (SHARED_MIN_ROWS_FEW if self.table.batch > 2 and self.table.batch * group <= 16 else SHARED_MIN_ROWS):
+        if saved < (SHARED_MIN_ROWS_FEW if self.table.batch * group <= 16 else SHARED_MIN_ROWS):
             return None
         return (streams.get(_lib.raw_stream(self.device.index))
                 or _lib.per_stream(streams, self.device.index, lambda: _upload((head, own, cnt), self.device)))
