@@ -185,3 +185,36 @@ def test_shared_entry_refusals():
     assert pages(table=4104) == pages(own=4104) == _lib.TC_ERR_ALIGNMENT
     assert pages(kn=4096) == pages(kn=4096, vn=4096, max_tiles=0) == _lib.TC_ERR_INVALID_ARGUMENT
     assert pages(kn=4100, vn=4096) == _lib.TC_ERR_ALIGNMENT
+
+
+@pytest.mark.parametrize("n", [1, 3, 16, 40])
+def test_a_step_reserves_what_each_sequence_would(n):
+    """reserve_all against reserve on an equal table, from empty sequences, shared and full last pages on."""
+    tables = [PageTable(300, 16, 4) for _ in range(2)]
+    for t in tables:
+        t.reserve(0, 33)
+        t.fork(0, 1, 33)
+        t.reserve(2, 32)
+    for step in range(12):
+        a, b = tables
+        if step == 5:
+            for t in tables:
+                t.release(1)
+        starts = [a.length(i) for i in range(4)]
+        rows = a.reserve_all(n)
+        assert rows.dtype == np.int32 and rows.shape == (4, n, 4)
+        for i in range(4):
+            assert np.array_equal(rows[i, :, :2], b.reserve(i, n))
+            assert rows[i, :, 2].tolist() == list(range(starts[i], starts[i] + n)) and not rows[i, :, 3].any()
+            assert a.length(i) == b.length(i) == starts[i] + n == int(a.frags[i][:, 2].sum())
+            assert np.array_equal(a.frags[i], b.frags[i])
+        assert a.free == b.free and a.users == b.users
+        if step % 3 == 2:  # the last token goes again
+            for t in tables:
+                for i in range(4):
+                    t.prune(i, t.length(i) - 1, t.length(i), 0)
+    short = PageTable(4, 16, 2)
+    short.reserve(0, 16)
+    with pytest.raises(RuntimeError, match="pages needed"):
+        short.reserve_all(33)
+    assert short.length(0) == 16 and short.length(1) == 0 and len(short.free) == 3

@@ -177,6 +177,7 @@ class PageTable:
         self.page_tokens = int(page_tokens)
         self.free = list(range(self.num_pages - 1, -1, -1))  # pop() hands out the lowest id first
         self.frags = [_EMPTY.copy() for _ in range(batch)]
+        self._lengths = {}  # (the fragments it was counted from, tokens) of each sequence
         self.users = {}  # pages that more than one sequence uses (fork): how many do
         self.version = 0  # bumped on every change, so device copies know when to refresh
 
@@ -185,7 +186,18 @@ class PageTable:
         return len(self.frags)
 
     def length(self, b):
-        return int(self.frags[b][:, 2].sum())
+        known, fr = self._lengths.get(b), self.frags[b]
+        if known is None or known[0] is not fr:  # (fragments are replaced, never changed in place)
+            known = self._lengths[b] = (fr, int(fr[:, 2].sum()))
+        return known[1]
+
+    def _extend(self, b, n):
+        """n tokens more (or fewer) on the last page of sequence b."""
+        length, fr = self.length(b) + n, self.frags[b].copy()
+        fr[-1, 2] += n
+        self.frags[b] = fr
+        self._lengths[b] = (fr, length)
+        self.version += 1
 
     def _room(self, b):
         """Slots that sequence b's next tokens find on its last page (none on a shared one: the others' tokens are,
@@ -233,9 +245,7 @@ class PageTable:
         room = self._room(b)
         if 0 < n <= room:  # the usual step: behind the last token
             page, first, count = fr[-1].tolist()
-            self.frags[b] = fr = fr.copy()
-            fr[-1, 2] = count + n
-            self.version += 1
+            self._extend(b, n)
             out = np.empty((n, 2), dtype=np.int64)
             out[:, 0] = page
             out[:, 1] = np.arange(first + count, first + count + n)
@@ -264,6 +274,24 @@ class PageTable:
         self.version += 1
         return out
 
+    def reserve_all(self, n):
+        """Slots of the next n tokens of every sequence, rows (page, slot, position, 0), int32 [B, n, 4]. Without room
+        for all of them nothing is reserved."""
+        n, P = int(n), self.page_tokens
+        at = [(*fr[-1].tolist(), self.length(b)) if len(fr) else (-1, 0, P, 0) for b, fr in enumerate(self.frags)]
+        if all(first + count + n <= P and page not in self.users for page, first, count, _ in at):  # the usual step
+            out = np.zeros((self.batch, n, 4), dtype=np.int32)
+            out[:, :, :3] = np.array([(page, first + count, start) for page, first, count, start in at])[:, None]
+            if n > 1:
+                out[:, :, 1:3] += np.arange(n)[:, None]
+            for b in range(self.batch):
+                self._extend(b, n)
+            return out
+        need = sum(self.pages_needed(b, n) for b in range(self.batch))
+        if need > len(self.free):
+            raise RuntimeError(f"PageTable: {need} pages needed, {len(self.free)} free")
+        return np.stack([_placed(self.reserve(b, n), start) for b, (*_, start) in enumerate(at)])
+
     def prune(self, b, a, c0, c):
         """Keep tokens [0, a) and [c0, c0 + c) of sequence b; returns (the kept
         suffix's fragments, the pages freed) (tc_page_prune)."""
@@ -272,9 +300,7 @@ class PageTable:
         if not (0 <= a <= c0 and c >= 0 and c0 + c <= n):
             raise ValueError(f"prune: split (a={a}, c0={c0}, c={c}) outside a sequence of {n} tokens")
         if c == 0 and len(old) and n - int(old[-1, 2]) < a:  # last tokens of the last fragment go: it keeps its page
-            self.frags[b] = old = old.copy()
-            old[-1, 2] -= n - a
-            self.version += 1
+            self._extend(b, a - n)
             return _EMPTY.copy(), []
         f, fp, nf = _frag_arg(old)
         # One buffer: kept (nf + 1 rows), suffix (nf rows), freed (nf), counts (3).
@@ -312,9 +338,11 @@ class PageTable:
         `window` tokens and its first `sink_tokens`; with `skip`, without its first `skip`
         fragments (the same in every sequence)."""
         lib, B = _lib.load(), self.batch
-        frags = [_frag_arg(f) for f in self.frags]
-        # One array of what the call reads: the lists' addresses, then their lengths.
-        args = np.array([a + 24 * skip for _, a, _ in frags] + [n - skip for _, _, n in frags], dtype=np.int64)
+        # One array of what the call reads, the lists' addresses and then their lengths, over one array of the lists.
+        frags, args = np.concatenate(self.frags, dtype=np.int64), np.empty((2, B), dtype=np.int64)
+        args[1] = [len(f) for f in self.frags]
+        args[0] = _addr(frags) + 24 * (args[1].cumsum() - args[1] + skip)
+        args[1] -= skip
         base = _addr(args)
         start = int(self.frags[0][:skip, 2].sum()) if skip else 0
         fixed = (base, base + 8 * B, B, self.page_tokens, start, min(int(window or 0), 1 << 40),
@@ -757,15 +785,9 @@ class PagedKV:
         if n < 1:
             raise ValueError(f"PagedKV.reserve_step: {n} tokens")
         self._refuse_during_step("reserve_step")
-        need = sum(self.table.pages_needed(b, n) for b in range(self.table.batch))
-        if need > len(self.table.free):
-            raise RuntimeError(f"PagedKV.reserve_step: {need} pages needed, {len(self.table.free)} free")
-        slots = []
-        for b in range(self.table.batch):
-            start = self.table.length(b)
-            slots.append(_placed(self.table.reserve(b, n), start))
+        slots = self.table.reserve_all(n)
         # (table version, layers not written yet, tokens, the slots and their copy for each stream)
-        self._step = (self.table.version, set(range(self.layers)), int(n), np.stack(slots), {})
+        self._step = (self.table.version, set(range(self.layers)), int(n), slots, {})
 
     def _step_slots(self, step):
         """The reserved step's slots on the device (int32 [B, n, 4])."""
