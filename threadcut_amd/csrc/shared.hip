@@ -20,6 +20,11 @@
 //     k indices are, for lane group g, the tokens 4g .. 4g + 3 of both tiles:
 //     P^T leaves the S^T registers without moving between lanes, V^T comes from
 //     the wave's LDS region by the transposing read, once for all blocks.
+//
+// Bound: HBM for few columns (16 over 10000 tokens of 8 heads, 200 to 500
+// own tokens each: 15.5 us with the combine, 47 MB); for many the vector instructions of the softmax
+// beside the products (512 columns over 16384 tokens of 8 heads: 81 us, of which
+// reading once would take 52; its products alone 25).
 #include <algorithm>
 
 #include "decode_tile.hpp"
@@ -378,7 +383,10 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
     __syncthreads();  // the one that the other half of the work-group meets in its merge
 }
 
-// The shape of a call: all columns in one work-group up to 256, else in blocks of them.
+// The shape of a call: all columns in one work-group up to 256, else in blocks of them, and no more column groups than
+// they fill, so that the rest of the waves share the keys. Against the next larger shape (us, 8 heads of 4 rows, 200 own
+// tokens, prefixes of 2048 and 16384): 16 columns 8.0 and 18.6, 9.3 and 20.5; 32: 10.8 and 21.8, 11.1 and 19.8 (but
+// with the weights rounded once); 64: 13.1 and 22.1, 11.9 and 23.8; 128: 16.9 and 31.7, 16.5 and 34.6.
 struct Plan {
   int cg, r;
   int64_t blocks;
