@@ -420,3 +420,21 @@ def test_no_query_heads(gpu, monkeypatch):
         c.fork(0, i)
     with pytest.raises((ValueError, RuntimeError)):
         c.decode(0, x.new_empty(3, 8, 0, D), SCALE)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("b,hkv,g,prefix,most", [(300, 1, 5, 700, 33), (43, 3, 8, 1234, 400), (130, 8, 1, 5, 16), (128, 8, 1, 3000, 0)])
+def test_many_rows(gpu, dtype, b, hkv, g, prefix, most):
+    """1024 rows and more, which another kernel joins: rows that do not fill a work-group, sequences without own tokens,
+    outputs whose heads are not next to each other, their neighbours left as they were."""
+    lens = [(7 * i) % (most + 1) for i in range(b)]
+    kp, vp = (rand(i, (hkv, prefix, D), dtype, gpu) for i in range(2))
+    k, v = (rand(5 + i, (b, hkv, most, D), dtype, gpu) for i in range(2))
+    q = rand(3, (b, hkv, g, D), dtype, gpu)
+    t = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    buf = torch.full((b, g, hkv + 1, D + 8), 7.0, dtype=dtype, device=gpu)
+    out = buf[:, :, :hkv, :D].transpose(1, 2)
+    assert flash_decode.decode_attention_shared(q, kp, vp, k, v, SCALE, lens=t, out=out) is out
+    check(out, q, kp, vp, k, v, lens)
+    buf[:, :, :hkv, :D] = 7.0
+    assert torch.all(buf == 7.0)

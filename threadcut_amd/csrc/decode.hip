@@ -901,6 +901,12 @@ struct Prefix {
   const int32_t* tiles = nullptr;
 };
 
+// Many rows with few splits are joined by the kernel that gives a row to half a wave: the combine kernel's four waves a
+// row, which read 32 splits at once, then cost their dispatch. Whole calls (us; the combine kernel's first): 4096 rows of
+// 9 splits 84.5, 80.4; 4096 of 3 59.0, 52.9; 1024 of 9 34.8, 34.1; 768 of 14 the same; 512 of 15 13.2, 13.8; 1024 of 20
+// 32.0, 32.6; 1280 of 25 29.5, 30.0; 128 of 29 18.3, 19.9.
+constexpr int kJoinRows = 1024, kJoinSplits = 16;
+
 // Splits of a shared-prefix call: the prefix's come first.
 int shared_plan(int batch, int kv_heads, int group, int64_t prefix_tokens, int64_t max_tokens, int ragged, int* S_prefix,
                 int* S_own, int* T_own) {
@@ -987,6 +993,11 @@ int shared_impl(const void* q_dev, const int64_t q_strides[3], const Prefix& x, 
   const int64_t shares = int64_t(Sp) * ceil_div(int64_t(batch) * group, 256) + int64_t(S) * batch;
   if (shares * kv_heads > 0x7fffffff) return fail(TC_ERR_UNSUPPORTED, "grid too large");
   if ((rc = hip_status(launch_shared(a, own, dtype, static_cast<hipStream_t>(stream)), "shared-prefix launch")) != TC_OK) return rc;
+  if (int64_t(batch) * kv_heads * group >= kJoinRows && Sp + S <= kJoinSplits) {
+    const JoinArgs j{o_part, lse_part, static_cast<uint16_t*>(out_dev), out_strides[0], out_strides[1], out_strides[2],
+                     kv_heads, group, batch, Sp + S};
+    return hip_status(launch_join(j, dtype, static_cast<hipStream_t>(stream)), "shared-prefix join launch");
+  }
   return tc_decode_combine(o_part, lse_part, batch, kv_heads, group, head_dim, Sp + S, out_dev, out_strides, dtype,
                            stream);
 }

@@ -383,6 +383,52 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
     __syncthreads();  // the one that the other half of the work-group meets in its merge
 }
 
+// A row (one query head of one sequence) takes 32 lanes, 4 dims each; a work-group 8 rows of one KV head. Its splits are
+// read 8 at a time, all before the first is used.
+template <int DT>
+__global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
+  using E = Elem<DT>;
+  constexpr int kPer = 8;
+  const int row = blockIdx.y * 8 + threadIdx.x / 32, d = 4 * (threadIdx.x % 32), h = blockIdx.x;
+  if (row >= a.batch * a.group) return;
+  const int b = row / a.group, g = row - b * a.group, S = a.splits;
+  const int64_t first = (static_cast<int64_t>(b) * a.heads + h) * S * a.group + g;
+  const float* const o = a.o_part + first * kHeadDim + d;
+  const float* const lse = a.lse_part + first;
+  float m = neg_inf(), L = 0.f;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < S; s0 += kPer) {
+    float4 v[kPer];
+    float x[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int64_t at = static_cast<int64_t>(min(s0 + j, S - 1)) * a.group;
+      v[j] = *reinterpret_cast<const float4*>(o + at * kHeadDim);
+      x[j] = lse[at];
+    }
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (s0 + j >= S) x[j] = neg_inf();
+      mn = fmaxf(mn, x[j]);
+    }
+    const float ms = mn == neg_inf() ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f((m - ms) * kLog2e);  // 0 while nothing was seen
+    m = mn;
+    L *= f;
+    O.x *= f; O.y *= f; O.z *= f; O.w *= f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const float w = __builtin_amdgcn_exp2f((x[j] - ms) * kLog2e);
+      L += w;
+      O.x += w * v[j].x; O.y += w * v[j].y; O.z += w * v[j].z; O.w += w * v[j].w;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that saw nothing is zero
+  *reinterpret_cast<uint2*>(a.out + b * a.so_b + h * a.so_h + g * a.so_g + d) =
+      make_uint2(E::bits(O.x * inv) | (E::bits(O.y * inv) << 16), E::bits(O.z * inv) | (E::bits(O.w * inv) << 16));
+}
+
 // The shape of a call: all columns in one work-group up to 256, else in blocks of them, and no more column groups than
 // they fill, so that the rest of the waves share the keys. Against the next larger shape (us, 8 heads of 4 rows, 200 own
 // tokens, prefixes of 2048 and 16384): 16 columns 8.0 and 18.6, 9.3 and 20.5; 32: 10.8 and 21.8, 11.1 and 19.8 (but
@@ -455,6 +501,15 @@ void shared_splits(int batch, int heads, int group, int64_t prefix_tiles, int64_
   const int64_t left = std::max<int64_t>(cus - sp * per_split, cus / 8) * (p.cg == 1 ? 1 : 2);
   *prefix = static_cast<int>(sp);
   *own = static_cast<int>(tiles ? std::max<int64_t>(1, std::min<int64_t>({(left + pairs / 2) / pairs, ceil_div(tiles, 4), 1024})) : 0);
+}
+
+hipError_t launch_join(const JoinArgs& a, int dtype, hipStream_t stream) {
+  const dim3 grid(a.heads, static_cast<unsigned>(ceil_div(int64_t(a.batch) * a.group, 8)));
+  if (dtype == TC_DTYPE_F16)
+    hipLaunchKernelGGL((join_kernel<TC_DTYPE_F16>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((join_kernel<TC_DTYPE_BF16>), grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
 }
 
 hipError_t launch_shared(const PrefixArgs& a_in, const PartialArgs& o, int dtype, hipStream_t stream) {

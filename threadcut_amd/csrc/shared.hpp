@@ -33,6 +33,16 @@ struct PrefixArgs {
 void shared_splits(int batch, int heads, int group, int64_t prefix_tiles, int64_t own_tokens, bool ragged, int cus,
                    int* prefix, int* own);
 
+// Joins the splits of a call with many rows (sequences x query heads): out_b from o_part and lse_part.
+struct JoinArgs {
+  const float* o_part;      // [B, H, S, G, D]
+  const float* lse_part;    // [B, H, S, G]
+  uint16_t* out;
+  int64_t so_b, so_h, so_g;
+  int heads, group, batch, splits;
+};
+hipError_t launch_join(const JoinArgs& a, int dtype, hipStream_t stream);
+
 // The launch: a for the prefix; o (its splits from a.splits on) for the own tokens, whose splits may be 0.
 hipError_t launch_shared(const PrefixArgs& a, const PartialArgs& o, int dtype, hipStream_t stream);
 
