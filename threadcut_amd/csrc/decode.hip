@@ -93,7 +93,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PAGED ? 
   __shared__ float s_acc[W][8][kHeadDim + 16];
   __shared__ float s_m[8][W];
   __shared__ float s_l[8][W];
-  decode_partial<DT, PAGED, APPEND, DIRECT, W, WINDOW>(a, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, threadIdx.x, s_vt,
+  decode_partial<DT, PAGED, APPEND, DIRECT, W, WINDOW, false>(a, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, threadIdx.x, s_vt,
                                                        s_acc, s_m, s_l);
 }
 
@@ -424,7 +424,7 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
                  int kv_heads, int group, int head_dim, int dtype, float scale, int split_tokens, int num_splits,
                  float* o_part_dev, float* lse_part_dev, int interleave, const Append* app, void* stream,
                  const Paged* paged = nullptr, bool whole_call = false, void* out_dev = nullptr,
-                 const int64_t* out_strides = nullptr, const Window* window = nullptr, int part0 = 0,
+                 const int64_t* out_strides = nullptr, const Window* window = nullptr,
                  PartialArgs* only = nullptr) {
   int rc = check_common(batch, kv_heads, group, head_dim, dtype);
   if (rc != TC_OK) return rc;
@@ -474,8 +474,7 @@ int partial_impl(const void* q_dev, const int64_t q_strides[3], const void* k_de
   a.group = group;
   a.splits = num_splits;
   a.split_tokens = split_tokens;
-  a.part0 = part0;
-  a.part_splits = part0 + num_splits;
+  a.part_splits = num_splits;
   a.interleave = interleave;
   // Longest sequences first: only for per-sequence lengths of a contiguous
   // cache, and up to 64 sequences (one lane each).
@@ -960,7 +959,12 @@ int shared_impl(const void* q_dev, const int64_t q_strides[3], const Prefix& x, 
   PartialArgs own{};
   if (S > 0 && (rc = partial_impl(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, lens_dev, n_tokens, batch,
                                   kv_heads, group, head_dim, dtype, scale, t, S, o_part, lse_part, 1, app, stream,
-                                  paged, true, nullptr, nullptr, nullptr, Sp, &own)) != TC_OK) return rc;
+                                  paged, true, nullptr, nullptr, nullptr, &own)) != TC_OK) return rc;
+  if (S > 0) {  // their splits come after the prefix's
+    own.o_part += static_cast<int64_t>(Sp) * group * head_dim;
+    own.lse_part += static_cast<int64_t>(Sp) * group;
+    own.part_splits = Sp + S;
+  }
 #if TC_DECODE_STAMPS
   own.stamps = nullptr;  // the timeline's buffer is laid out for the decode partial kernel's grid
 #endif

@@ -160,15 +160,14 @@ struct PartialArgs {
   const uint16_t* q;
   const uint16_t* k;
   const uint16_t* v;
-  float* o_part;       // [B, H, part_splits, G, D]: this call's splits from part0 on
-  float* lse_part;     // [B, H, part_splits, G]
+  float* o_part;       // [B, H, S, G, D]
+  float* lse_part;     // [B, H, S, G]
   const int32_t* lens; // [B] or null
   int64_t n;
   int64_t sq_b, sq_h, sq_g;
   int64_t sk_b, sk_h, sk_t;
   int64_t sv_b, sv_h, sv_t;
   int heads, group, splits, split_tokens;
-  int part_splits, part0;
   int interleave;      // 0: split s owns tokens [s*T, (s+1)*T); 1: 16-token tiles dealt round-robin
   int longest_first;   // per-sequence lengths, batch <= 64: work-group row z serves the z-th longest sequence
   float scale_log2;    // softmax scale * log2(e)
@@ -197,13 +196,17 @@ struct PartialArgs {
   // into the head slab of the pools.
   const int32_t* tok_off;
   int64_t tok_pitch;
-  // Window (decode_partial_kernel<..., true>): sequence b's query sees its last
-  // `window` tokens, an appended one among them, and the first `sinks` ones.
-  int32_t window, sinks;
   // One split: the result itself, rounded to the element type as the combine
   // rounds it (null: the partial goes to o_part, lse_part).
   uint16_t* out;
   int64_t so_b, so_h, so_g;
+  // Window (decode_partial_kernel<..., true>): sequence b's query sees its last
+  // `window` tokens, an appended one among them, and the first `sinks` ones.
+  int32_t window, sinks;
+  // Beside another part's splits (decode_partial<..., true>): a (sequence,
+  // head) has part_splits of them in o_part and lse_part, which point at this
+  // call's first.
+  int part_splits;
 #if TC_DECODE_STAMPS
   // Per wave ((b * heads + h) * splits + split) * waves + wave, 8 words:
   // realtime-clock stamps (100 MHz) at the kernel's start, after the first
@@ -228,7 +231,7 @@ namespace {
 // The work of W waves, which may be a work-group of its own or a part of one (tid is the thread's index in it): head h's
 // split `split` of the z-th of `sequences` sequences. s_vt: the waves' V tiles; s_acc, s_m and s_l: the merge's rows,
 // padded by 16 words, so the float4 stores of the g heads (one head per 16 lanes) fall on distinct banks.
-template <int DT, bool PAGED, bool APPEND, bool DIRECT, int W, bool WINDOW>
+template <int DT, bool PAGED, bool APPEND, bool DIRECT, int W, bool WINDOW, bool BESIDE>
 __device__ __forceinline__ void decode_partial(const PartialArgs& a, const int h, const int split, const int z,
                                                const int sequences, const int tid, uint32_t (*s_vt)[kVTileWords],
                                                float (*s_acc)[8][kHeadDim + 16], float (*s_m)[W], float (*s_l)[W]) {
@@ -520,7 +523,7 @@ __device__ __forceinline__ void decode_partial(const PartialArgs& a, const int h
 #endif
   // The head's sum over the four lane groups; m is already common to them.
   l = rows_sum(l);
-  const int64_t part = (static_cast<int64_t>(b) * a.heads + h) * a.part_splits + a.part0 + split;
+  const int64_t part = (static_cast<int64_t>(b) * a.heads + h) * (BESIDE ? a.part_splits : a.splits) + split;
   static_assert(W > 1, "the waves of a work-group are merged below");
   if (n < a.group) {
 #pragma unroll

@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * S::W) __attribute__((amdgpu_waves_per_eu(S::W 
   static_assert(2 * 8 * kOwn <= S::W / kUnits * 16, "a share's maxima and sums");
   float* const ml = unit ? s_l[0] : s_m[0];
   if (z < static_cast<uint32_t>(a.batch))
-    decode_partial<DT, PAGED, APPEND, false, kOwn, false>(
+    decode_partial<DT, PAGED, APPEND, false, kOwn, false, true>(
         o, h, j - z * o.splits, z, a.batch, threadIdx.x - unit * 64 * kOwn, reinterpret_cast<uint32_t(*)[kVTileWords]>(vt),
         reinterpret_cast<float(*)[8][kHeadDim + 16]>(acc), reinterpret_cast<float(*)[kOwn]>(ml),
         reinterpret_cast<float(*)[kOwn]>(ml + 8 * kOwn));
