@@ -734,10 +734,11 @@ class PagedKV:
             # The whole call in native code; None for what it does not take (then as below).
             stream = _lib.raw_stream(self.device.index)
             key = (self.table.version, window, sink_tokens, stream, q.shape[2])
-            if self._last_tables[0] != key:  # the layers of a step ask for the same ones
+            last = self._last_tables  # (read once: another thread may replace it)
+            if last[0] != key:  # the layers of a step ask for the same ones
                 shared = self.shared_tables(q.shape[2]) if window is None else None
-                self._last_tables = (key, shared, None if shared else self.window_table(window, sink_tokens, "decode"))
-            _, shared, table = self._last_tables
+                last = self._last_tables = (key, shared, None if shared else self.window_table(window, sink_tokens, "decode"))
+            _, shared, table = last
             if shared:
                 done = fast.paged_shared(q, self.k_pools[layer], self.v_pools[layer], *shared, None, None, out, scale,
                                          stream)
