@@ -674,10 +674,8 @@ class PagedKV:
             mptr, mst = m.data_ptr(), pf._mask_strides(m)
         lib = _lib.load()
         kp, vp = self.k_pools[layer], self.v_pools[layer]
-        with torch.cuda.device(self.device):
-            splits = (pf.num_splits(b, ql, n, hq, self.kv_heads) if w is None
-                      else pf.window_splits(b, ql, n, *w, hq, self.kv_heads))
-            nbytes = lib.tc_prefill_workspace_bytes(b, ql, hq, splits)
+        splits, nbytes = pf._plan(self.device.index, b, ql, n, w, hq, self.kv_heads)
+        with _on_device(self.device):
             ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
             if w is not None:
                 rc = lib.tc_prefill_paged_window_attention(

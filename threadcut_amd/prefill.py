@@ -9,11 +9,13 @@ K and V in LDS once for all of them and runs QKᵀ and PV on the matrix cores wi
 online softmax. This module checks tensors and passes pointers, strides and
 the current stream.
 """
+import functools
 import weakref
 
 import torch
 
 from . import _lib
+from .flash_decode import _on_device
 
 HEAD_DIM = 128
 GROUPS = (1, 2, 4, 8)
@@ -74,6 +76,16 @@ def window_splits(batch, q_len, n_tokens, window, sink_tokens, q_heads, kv_heads
     return s
 
 
+@functools.lru_cache(maxsize=1024)
+def _plan(device_index, batch, q_len, n_tokens, window, q_heads, kv_heads, splits=0):
+    """(splits, workspace bytes) of a call, windowed or not: the plan depends on the device's compute units, so it is
+    made with that device current, once for the layers of a step."""
+    with torch.cuda.device(device_index):
+        s = splits or (num_splits(batch, q_len, n_tokens, q_heads, kv_heads) if window is None
+                       else window_splits(batch, q_len, n_tokens, *window, q_heads, kv_heads))
+    return s, _lib.load().tc_prefill_workspace_bytes(batch, q_len, q_heads, s)
+
+
 def prefill_attention(query, key, value, attention_mask=None, scale=None, is_causal=False, out=None, splits=None,
                       window=None, sink_tokens=0):
     """SDPA(query, repeat_kv(key, g), repeat_kv(value, g), attention_mask, scale,
@@ -124,10 +136,8 @@ def prefill_attention(query, key, value, attention_mask=None, scale=None, is_cau
         mask_ptr, mask_strides = m.data_ptr(), _mask_strides(m)
     scale = scale if scale is not None else d ** -0.5
     lib = _lib.load()
-    # The library plans splits for the current device (its CU count).
-    with torch.cuda.device(query.device):
-        s = int(splits) if splits else num_splits(b, q, n, hq, hkv) if w is None else window_splits(b, q, n, *w, hq, hkv)
-        ws_bytes = lib.tc_prefill_workspace_bytes(b, q, hq, s)
+    s, ws_bytes = _plan(query.get_device(), b, q, n, w, hq, hkv, int(splits or 0))
+    with _on_device(query.device):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
         if w is not None:
             rc = lib.tc_prefill_window_attention(
